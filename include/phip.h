@@ -641,6 +641,124 @@ int phip_max_pool2d_bw_bf16(phip_ctx *ctx, const void *x, const void *y, const v
     uint32_t x1, uint32_t repeat, uint32_t win0, uint32_t win1, uint32_t pad0, uint32_t pad1, uint32_t str0,
     uint32_t str1);
 
+/* ---- sequences of a minibatch -------------------------------------------------
+ * No counterpart in the reference, which unrolls sequences in its graph
+ * (examples/ptb/ptb_rnnlm_lstm.cc:146-154).  The operators below work on
+ * tensors of [d, heads, tokens] x batch (first index fastest).  A list of
+ * sequences says which tokens are used:
+ *   packed == 0: sequence i is the first q_lens[i] of the tq tokens of sample i
+ *                (of queries) and the first k_lens[i] of its tk tokens (of
+ *                keys, e.g. the filled part of a cache); n is the batch size;
+ *   packed != 0: the sequences lie one after another in one sample, in the
+ *                order of the list.
+ * k_lens == NULL: as q_lens.  Lengths may be 0.  The queries of a sequence are
+ * its LAST q_lens[i] tokens: their positions are k_lens[i] - q_lens[i] and up.
+ * A call that gets NULL instead of a list takes every sample whole, with its
+ * first token at position 0 (attention: with the queries as the last tq of
+ * the tk tokens).
+ * The lengths are HOST arrays, copied by the call, which does not wait for the
+ * GPU.  One list serves any number of calls (every layer, both directions) of
+ * the context that made it; it is destroyed before or after that context, and
+ * at any time after the calls that read it were made. */
+typedef struct phip_sequences phip_sequences;
+int phip_sequences_create(phip_ctx *ctx, const uint32_t *q_lens, const uint32_t *k_lens, uint32_t n, int packed,
+                          phip_sequences **out);
+int phip_sequences_destroy(phip_sequences *seqs);
+
+/* ---- rotary positions ----------------------------------------------------------
+ * No counterpart in the reference.  Rotates the first 2*pairs elements of each
+ * head of the queries xq ([d, hq, t] x bs) and of the keys xk ([d, hk, t] x bs;
+ * NULL with hk == 0: queries only) of the same tokens, pair i by the angle
+ * position * freqs[i] (the product is exact: far positions lose nothing), and
+ * copies the rest of the head.  Pair i is (x[i], x[i + pairs]), or with
+ * interleaved != 0 (x[2i], x[2i+1]); the rotated elements are scaled by
+ * `amplitude` (1 for plain rotation).  freqs: HOST array of `pairs` values.  The
+ * position of a token is first + its position in its sequence (`seqs`; NULL:
+ * its index in the sample).  d <= 128.
+ * Forward overwrites; tokens that belong to no sequence get zeros.  A result may
+ * take its own operand's place.  Backward: gx += the rotation by the opposite
+ * angle of gy, nothing for tokens of no sequence. */
+int phip_rotary_fw_f32(phip_ctx *ctx, const float *xq, const float *xk, float *yq, float *yk, uint32_t d, uint32_t hq,
+    uint32_t hk, uint32_t t, uint32_t bs, const phip_sequences *seqs, int32_t first, const float *freqs,
+    uint32_t pairs, int interleaved, float amplitude);
+int phip_rotary_fw_f16(phip_ctx *ctx, const void *xq, const void *xk, void *yq, void *yk, uint32_t d, uint32_t hq,
+    uint32_t hk, uint32_t t, uint32_t bs, const phip_sequences *seqs, int32_t first, const float *freqs,
+    uint32_t pairs, int interleaved, float amplitude);
+int phip_rotary_fw_bf16(phip_ctx *ctx, const void *xq, const void *xk, void *yq, void *yk, uint32_t d, uint32_t hq,
+    uint32_t hk, uint32_t t, uint32_t bs, const phip_sequences *seqs, int32_t first, const float *freqs,
+    uint32_t pairs, int interleaved, float amplitude);
+int phip_rotary_bw_f32(phip_ctx *ctx, const float *gyq, const float *gyk, float *gxq, float *gxk, uint32_t d, uint32_t hq,
+    uint32_t hk, uint32_t t, uint32_t bs, const phip_sequences *seqs, int32_t first, const float *freqs,
+    uint32_t pairs, int interleaved, float amplitude);
+int phip_rotary_bw_f16(phip_ctx *ctx, const void *gyq, const void *gyk, void *gxq, void *gxk, uint32_t d, uint32_t hq,
+    uint32_t hk, uint32_t t, uint32_t bs, const phip_sequences *seqs, int32_t first, const float *freqs,
+    uint32_t pairs, int interleaved, float amplitude);
+int phip_rotary_bw_bf16(phip_ctx *ctx, const void *gyq, const void *gyk, void *gxq, void *gxk, uint32_t d, uint32_t hq,
+    uint32_t hk, uint32_t t, uint32_t bs, const phip_sequences *seqs, int32_t first, const float *freqs,
+    uint32_t pairs, int interleaved, float amplitude);
+
+/* The same behind a norm of each head, in one pass: n = x * w / sqrt(mean(x^2) +
+ * eps) over the d elements of a head, with weights wq for queries and wk for
+ * keys ([d] each), then the rotation of n.  Backward: gx += and gw += (a
+ * weight's gradient collects every token and head, in a fixed order). */
+int phip_norm_rotary_fw_f32(phip_ctx *ctx, const float *xq, const float *xk, const float *wq, const float *wk, float *yq,
+    float *yk, uint32_t d, uint32_t hq, uint32_t hk, uint32_t t, uint32_t bs, const phip_sequences *seqs,
+    int32_t first, const float *freqs, uint32_t pairs, int interleaved, float amplitude, float eps);
+int phip_norm_rotary_fw_f16(phip_ctx *ctx, const void *xq, const void *xk, const void *wq, const void *wk, void *yq,
+    void *yk, uint32_t d, uint32_t hq, uint32_t hk, uint32_t t, uint32_t bs, const phip_sequences *seqs,
+    int32_t first, const float *freqs, uint32_t pairs, int interleaved, float amplitude, float eps);
+int phip_norm_rotary_fw_bf16(phip_ctx *ctx, const void *xq, const void *xk, const void *wq, const void *wk, void *yq,
+    void *yk, uint32_t d, uint32_t hq, uint32_t hk, uint32_t t, uint32_t bs, const phip_sequences *seqs,
+    int32_t first, const float *freqs, uint32_t pairs, int interleaved, float amplitude, float eps);
+int phip_norm_rotary_bw_f32(phip_ctx *ctx, const float *xq, const float *xk, const float *wq, const float *wk,
+    const float *gyq, const float *gyk, float *gxq, float *gxk, float *gwq, float *gwk, uint32_t d, uint32_t hq,
+    uint32_t hk, uint32_t t, uint32_t bs, const phip_sequences *seqs, int32_t first, const float *freqs,
+    uint32_t pairs, int interleaved, float amplitude, float eps);
+int phip_norm_rotary_bw_f16(phip_ctx *ctx, const void *xq, const void *xk, const void *wq, const void *wk,
+    const void *gyq, const void *gyk, void *gxq, void *gxk, void *gwq, void *gwk, uint32_t d, uint32_t hq,
+    uint32_t hk, uint32_t t, uint32_t bs, const phip_sequences *seqs, int32_t first, const float *freqs,
+    uint32_t pairs, int interleaved, float amplitude, float eps);
+int phip_norm_rotary_bw_bf16(phip_ctx *ctx, const void *xq, const void *xk, const void *wq, const void *wk,
+    const void *gyq, const void *gyk, void *gxq, void *gxk, void *gwq, void *gwk, uint32_t d, uint32_t hq,
+    uint32_t hk, uint32_t t, uint32_t bs, const phip_sequences *seqs, int32_t first, const float *freqs,
+    uint32_t pairs, int interleaved, float amplitude, float eps);
+
+/* ---- attention -------------------------------------------------------------------
+ * No counterpart in the reference, whose examples write it as matmul, softmax
+ * and matmul (examples/encdec/encdec_attention.cc) with every matrix of scores
+ * in memory.  y = softmax(scale * q k^T) v per sequence and head: q and y are
+ * [d, hq, tq] x bs, k and v [d, hk, tk] x bs, and each key head serves hq / hk
+ * consecutive query heads.  causal != 0: query i of lq sees the keys up to
+ * i + lk - lq of lk (the queries are the sequence's last tokens).  A row that
+ * sees no key gives 0, and so do tokens of no sequence; what k and v hold
+ * outside the sequences is never used.  d <= 128, scale > 0.
+ * stats (may be NULL): float [hq, tq] x bs, the logarithm of the sum of
+ * exponentials of each row, which the gradients need; -inf where no key is
+ * seen.  Few queries against many keys (the single tokens of a serving loop)
+ * split the keys between workgroups.
+ * Backward: gq, gk, gv += from q, k, v, the forward call's y and stats, and
+ * gy; the heads that share a key head add up in its gradient.  One tensor may
+ * be queries, keys and values: its gradient is then passed for each.  All sums
+ * are in fp32 and in a fixed order: the same bits on every run. */
+int phip_attention_fw_f32(phip_ctx *ctx, const float *q, const float *k, const float *v, float *y, float *stats,
+    uint32_t d, uint32_t hq, uint32_t hk, uint32_t tq, uint32_t tk, uint32_t bs, const phip_sequences *seqs,
+    int causal, float scale);
+int phip_attention_fw_f16(phip_ctx *ctx, const void *q, const void *k, const void *v, void *y, float *stats,
+    uint32_t d, uint32_t hq, uint32_t hk, uint32_t tq, uint32_t tk, uint32_t bs, const phip_sequences *seqs,
+    int causal, float scale);
+int phip_attention_fw_bf16(phip_ctx *ctx, const void *q, const void *k, const void *v, void *y, float *stats,
+    uint32_t d, uint32_t hq, uint32_t hk, uint32_t tq, uint32_t tk, uint32_t bs, const phip_sequences *seqs,
+    int causal, float scale);
+int phip_attention_bw_f32(phip_ctx *ctx, const float *q, const float *k, const float *v, const float *y,
+    const float *stats, const float *gy, float *gq, float *gk, float *gv, uint32_t d, uint32_t hq, uint32_t hk,
+    uint32_t tq, uint32_t tk, uint32_t bs, const phip_sequences *seqs, int causal, float scale);
+int phip_attention_bw_f16(phip_ctx *ctx, const void *q, const void *k, const void *v, const void *y,
+    const float *stats, const void *gy, void *gq, void *gk, void *gv, uint32_t d, uint32_t hq, uint32_t hk,
+    uint32_t tq, uint32_t tk, uint32_t bs, const phip_sequences *seqs, int causal, float scale);
+int phip_attention_bw_bf16(phip_ctx *ctx, const void *q, const void *k, const void *v, const void *y,
+    const float *stats, const void *gy, void *gq, void *gk, void *gv, uint32_t d, uint32_t hq, uint32_t hk,
+    uint32_t tq, uint32_t tk, uint32_t bs, const phip_sequences *seqs, int causal, float scale);
+
 /* ---- timing ---------------------------------------------------------------
  * No counterpart in the reference (it has no profiling facility); events are
  * recorded on the context's stream so they bracket exactly the kernels the

@@ -199,6 +199,8 @@ SIGNATURES = {
     "phip_conv2d_bw_bf16": [_vp, _vp, _vp, _vp, _vp, _vp] + [_u32] * 14,
     "phip_max_pool2d_fw_bf16": [_vp, _vp, _vp] + [_u32] * 9,
     "phip_max_pool2d_bw_bf16": [_vp, _vp, _vp, _vp, _vp] + [_u32] * 9,
+    "phip_sequences_create": [_vp, _ids, _ids, _u32, _int, _pp],
+    "phip_sequences_destroy": [_vp],
     "phip_event_create": [_vp, _pp],
     "phip_event_destroy": [_vp],
     "phip_event_record": [_vp, _vp],
@@ -208,6 +210,17 @@ SIGNATURES = {
     "phip_randomizer_fill_uniform": [_vp, _f, _f, _sz, _vp],
     "phip_randomizer_fill_normal": [_vp, _f, _f, _sz, _vp],
 }
+# d, hq, hk, t, bs, seqs, first, freqs, pairs, interleaved, amplitude
+_ROTARY = [_u32] * 5 + [_vp, ctypes.c_int32, ctypes.POINTER(_f), _u32, _int, _f]
+# d, hq, hk, tq, tk, bs, seqs, causal, scale
+_ATTENTION = [_u32] * 6 + [_vp, _int, _f]
+for _suffix in ("f32", "f16", "bf16"):
+    SIGNATURES["phip_rotary_fw_" + _suffix] = [_vp] * 5 + _ROTARY
+    SIGNATURES["phip_rotary_bw_" + _suffix] = [_vp] * 5 + _ROTARY
+    SIGNATURES["phip_norm_rotary_fw_" + _suffix] = [_vp] * 7 + _ROTARY + [_f]
+    SIGNATURES["phip_norm_rotary_bw_" + _suffix] = [_vp] * 11 + _ROTARY + [_f]
+    SIGNATURES["phip_attention_fw_" + _suffix] = [_vp] * 6 + _ATTENTION
+    SIGNATURES["phip_attention_bw_" + _suffix] = [_vp] * 10 + _ATTENTION
 _RESTYPES = {"phip_last_error": ctypes.c_char_p, "phip_ctx_id": _u64}
 
 _lib = None

@@ -33,6 +33,10 @@ SOURCES = [
     "phip_gemm_h16_skinny.hip",
     "phip_gemm_h16_big.hip",
     "phip_matmul.hip",
+    "phip_sequences.hip",
+    "phip_rotary.hip",
+    "phip_attention_fw.hip",
+    "phip_attention_bw.hip",
 ]
 
 # Packed-fp32 instruction selection is switched off for all device code.

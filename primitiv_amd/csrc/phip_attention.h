@@ -1,0 +1,445 @@
+// Shared pieces of the attention kernels (forward and gradients).
+//
+// Everything is built from 32 x 32 blocks of the matrix instructions, and every product is arranged so that its result
+// can be the right operand of the next one without leaving the registers.  A lane of a result block holds one column
+// (lane % 32) and the rows (i & 3) + 8 (i >> 2) + 4 (lane / 32), i < 16; a right operand over 16 of those rows wants 8 of
+// them from each half of the wavefront.  Which 8 does not matter as long as the left operand is read in the same order:
+// chunk c of 16 rows gives half h the rows 16 c + 4 h + j (j < 4) and 16 c + 8 + 4 h + (j - 4), which are the registers
+// 8 c + j.  So the scores are computed transposed (keys down, queries across): a lane then owns a query, the softmax
+// needs one exchange between the halves per tile, and exp(scores) is the right operand of the product with the values.
+//
+// The three storage types share the code.  A fragment is 8 elements per lane for one 16-deep step: one
+// v_mfma_f32_32x32x16 for 16-bit storage, eight v_mfma_f32_32x32x2_f32 for fp32.
+#ifndef PHIP_ATTENTION_H_
+#define PHIP_ATTENTION_H_
+
+#include <atomic>
+#include <initializer_list>
+
+#include "phip_internal.h"
+#include "phip_sequences.h"
+#include "phip_types.h"
+
+namespace phip {
+namespace attention {
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x8 __attribute__((ext_vector_type(8)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef _Float16 half8v __attribute__((ext_vector_type(8)));
+typedef __bf16 bf8v __attribute__((ext_vector_type(8)));
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
+constexpr uint32_t kOutOfRange = 0x80000000u;  // past the end of any buffer described here
+
+template <class T>
+__device__ inline __attribute__((address_space(3))) T *lds_ptr(uint32_t addr) {
+  return (__attribute__((address_space(3))) T *)(size_t)addr;
+}
+
+// ---- fragments ------------------------------------------------------------------------------------------------------
+
+template <typename T>
+struct Frag16 {
+  u32x4 v;  // elements 2 e, 2 e + 1 in v[e]
+};
+template <typename T>
+struct FragOf {
+  typedef Frag16<T> type;
+};
+template <>
+struct FragOf<float> {
+  typedef f32x8 type;
+};
+template <typename T>
+using Frag = typename FragOf<T>::type;
+
+__device__ inline void mma(f32x16 &c, const Frag16<bf16_t> &a, const Frag16<bf16_t> &b) {
+  c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf8v, a.v), __builtin_bit_cast(bf8v, b.v), c, 0, 0, 0);
+}
+__device__ inline void mma(f32x16 &c, const Frag16<f16_t> &a, const Frag16<f16_t> &b) {
+  c = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(half8v, a.v), __builtin_bit_cast(half8v, b.v), c, 0, 0, 0);
+}
+__device__ inline void mma(f32x16 &c, const f32x8 &a, const f32x8 &b) {
+#pragma unroll
+  for (int j = 0; j < 8; ++j) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[j], b[j], c, 0, 0, 0);
+}
+
+// Two values rounded to nearest even and packed, x0 in the low half.  Left to the compiler, which knows the distance that
+// a matrix instruction needs from the conversion that writes its operand.
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+template <typename T>
+__device__ inline uint32_t round_pair(float x0, float x1) {
+  const f32x2 x = {x0, x1};
+  if constexpr (__is_same(T, bf16_t)) {
+    typedef __bf16 pair __attribute__((ext_vector_type(2)));
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector(x, pair));
+  } else {
+    typedef _Float16 pair __attribute__((ext_vector_type(2)));
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector(x, pair));
+  }
+}
+
+// Registers 8 c .. 8 c + 7 of a block as the right operand of the next product.  16-bit storage rounds here: the matrix
+// instruction takes no wider operand, and the probabilities carry one rounding as a stored probability matrix would.
+template <typename T>
+__device__ inline Frag16<T> as_operand(const f32x16 &p, int c, Frag16<T> *) {
+  Frag16<T> f;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) f.v[e] = round_pair<T>(p[8 * c + 2 * e], p[8 * c + 2 * e + 1]);
+  return f;
+}
+__device__ inline f32x8 as_operand(const f32x16 &p, int c, f32x8 *) {
+  f32x8 f;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) f[j] = p[8 * c + j];
+  return f;
+}
+
+// ---- global memory --------------------------------------------------------------------------------------------------
+
+template <typename T>
+struct alignas(sizeof(T)) Chunk {  // 16 bytes at any address that suits the element
+  T v[16 / sizeof(T)];
+};
+
+// `n` valid elements (at most one 16-byte chunk) at p, zeros behind them.
+template <typename T>
+__device__ inline u32x4 load_chunk(const T *p, int n) {
+  constexpr int N = 16 / sizeof(T);
+  u32x4 r = {0, 0, 0, 0};
+  if (n >= N) {
+    __builtin_memcpy(&r, reinterpret_cast<const Chunk<T> *>(p), 16);
+  } else if (n > 0) {
+    T e[N] = {};
+#pragma unroll
+    for (int i = 0; i < N - 1; ++i)
+      if (i < n) e[i] = p[i];
+    __builtin_memcpy(&r, e, 16);
+  }
+  return r;
+}
+
+// A lane's 8 elements d0 .. d0 + 7 of a row of `d` elements, zeros behind the row's end or for an absent row.
+template <typename T>
+__device__ inline Frag16<T> load_frag(const T *row, bool valid, int d0, int d, Frag16<T> *) {
+  return {load_chunk(row + (valid ? d0 : 0), valid ? d - d0 : 0)};
+}
+__device__ inline f32x8 load_frag(const float *row, bool valid, int d0, int d, f32x8 *) {
+  const u32x4 lo = load_chunk(row + (valid ? d0 : 0), valid ? d - d0 : 0);
+  const u32x4 hi = load_chunk(row + (valid && d - d0 > 4 ? d0 + 4 : 0), valid ? d - d0 - 4 : 0);
+  f32x8 f;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const uint32_t l = lo[e], h = hi[e];  // a bit cast of a vector's element itself takes the first one
+    f[e] = __builtin_bit_cast(float, l);
+    f[e + 4] = __builtin_bit_cast(float, h);
+  }
+  return f;
+}
+
+template <typename T>
+__device__ inline float element(const Frag16<T> &f, int j) {
+  const uint32_t bits = (j & 1) ? f.v[j >> 1] >> 16 : f.v[j >> 1] & 0xffffu;
+  if constexpr (__is_same(T, bf16_t)) return __builtin_bit_cast(float, bits << 16);
+  else return to_f32(__builtin_bit_cast(f16_t, (uint16_t)bits));
+}
+__device__ inline float element(const f32x8 &f, int j) { return f[j]; }
+
+__device__ inline u32x4 buffer_words(const void *p, uint32_t bytes) {
+  const uint64_t a = reinterpret_cast<uint64_t>(p);
+  // the address is the same in all lanes, which the compiler cannot always see
+  u32x4 r = {(uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)a),
+             (uint32_t)__builtin_amdgcn_readfirstlane((int)((uint32_t)(a >> 32) & 0xffffu)), bytes, 0x00020000u};
+  return r;
+}
+
+// One 16-byte-per-lane buffer load whose destination is LDS: lane l's data lands at lds_addr + 16 l, zeros for lanes
+// past the end of the buffer.  Inline assembly keeps the compiler from waiting for it in front of every later LDS read;
+// the kernels wait themselves (wait_loads) before the barrier that publishes a tile.  m0 is scratch; the wait state
+// between its write and the load is the one the instruction set asks for.
+__device__ inline void lds_dma_b128(u32x4 rsrc, uint32_t lds_addr, uint32_t voffset) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
+               :
+               : "s"(lds_addr), "v"(voffset), "s"(rsrc)
+               : "memory");
+}
+template <int N>
+__device__ inline void wait_loads() {
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+}
+
+// ---- tiles in LDS ---------------------------------------------------------------------------------------------------
+//
+// A tile is ROWS rows of DP elements (the head size rounded up to a multiple of 32, zeros behind the row's end) at a
+// pitch of a power of two.  The 16-byte chunk c of a row sits at position c ^ swizzle(row), so that both the reads along
+// a row (16 consecutive rows, the same chunk) and the transposing reads (4 consecutive rows, 4 neighbouring chunks)
+// spread over all 64 banks.
+template <typename T, int DP>
+struct Tile {
+  static constexpr int kPitch = (DP <= 32 ? 32 : DP <= 64 ? 64 : 128) * (int)sizeof(T);  // bytes
+  static constexpr int kChunks = kPitch / 16;
+  static constexpr int kPerChunk = 16 / (int)sizeof(T);
+
+  __device__ static inline int swizzle(int row) {
+    if constexpr (kChunks >= 16) return ((row & 3) << 2) | ((row >> 2) & 3);
+    else if constexpr (kChunks == 8) return (((row >> 1) & 1) << 2) | ((row >> 2) & 3);
+    else return (row >> 2) & 3;
+  }
+
+  // What a lane adds to a tile's address for the reads along rows: row lane % 32 of a 32-row block, half lane / 32.
+  __device__ static inline uint32_t row_lane(int lane) {
+    const int row = lane & 31, h = lane >> 5;
+    const int c = sizeof(T) == 2 ? h : 2 * h;
+    return (uint32_t)(row * kPitch + ((c ^ swizzle(row)) << 4));
+  }
+  // Elements 16 c + 8 h .. + 7 of the lane's row of block `blk`; `at` = tile address + row_lane.
+  __device__ static inline Frag<T> row_frag(uint32_t at, int blk, int c) {
+    if constexpr (sizeof(T) == 2) {
+      const uint32_t a = (at ^ (uint32_t)(c << 5)) + (uint32_t)(blk * 32 * kPitch);
+      return {*lds_ptr<u32x4>(a)};
+    } else {
+      const uint32_t a = (at ^ (uint32_t)(c << 6));
+      const f32x4 lo = *lds_ptr<f32x4>(a + (uint32_t)(blk * 32 * kPitch));
+      const f32x4 hi = *lds_ptr<f32x4>((a ^ 16u) + (uint32_t)(blk * 32 * kPitch));
+      return {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+    }
+  }
+
+  // The same for the transposing reads: the fragment of column 32 db + lane % 32 over the 16 rows of chunk rc in the
+  // order described at the top (rows 16 rc + 4 h + j, then 16 rc + 8 + 4 h + j).
+  __device__ static inline uint32_t col_lane(int lane) {
+    const int h = lane >> 5;
+    if constexpr (sizeof(T) == 2) {
+      // ds_read_b64_tr_b16: of 16 lanes, lane 4 a + b receives element b of the 8 bytes that lanes a, 4 + a, 8 + a and
+      // 12 + a point to; lane s points to row 4 h + s / 4, columns 4 (s % 4) .. + 3 of its 16
+      const int s = lane & 15, row = 4 * h + (s >> 2), col = 16 * ((lane >> 4) & 1) + 4 * (s & 3);
+      return (uint32_t)(row * kPitch + (((col >> 3) ^ swizzle(row)) << 4) + (col & 7) * 2);
+    } else {
+      const int row = 4 * h, col = lane & 31;
+      return (uint32_t)(row * kPitch + (((col >> 2) ^ swizzle(row)) << 4) + (col & 3) * 4);
+    }
+  }
+  __device__ static inline Frag<T> col_frag(uint32_t at, int rc, int db) {
+    if constexpr (sizeof(T) == 2) {
+      // rows 8 further on: the swizzle's low bits move by 2
+      const uint32_t a = (at ^ (uint32_t)(db << 6)) + (uint32_t)(16 * rc * kPitch);
+      const uint32_t b = (at ^ (uint32_t)(db << 6) ^ 32u) + (uint32_t)((16 * rc + 8) * kPitch);
+      const u32x2 lo = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(lds_ptr<s16x4>(a)));
+      const u32x2 hi = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(lds_ptr<s16x4>(b)));
+      return {{lo[0], lo[1], hi[0], hi[1]}};
+    } else {
+      f32x8 f;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const int row = 16 * rc + (j & 3) + 8 * (j >> 2);  // + 4 h, which is in `at`
+        f[j] = *lds_ptr<float>((at ^ (uint32_t)(db << 7) ^ flip(j)) + (uint32_t)(row * kPitch));
+      }
+      return f;
+    }
+  }
+  // (fp32) swizzle(4 h + row offset of element j) ^ swizzle(4 h), in bytes: the same for both halves
+  __device__ static inline uint32_t flip(int j) {
+    const int off = (j & 3) + 8 * (j >> 2);
+    if constexpr (kChunks >= 16) return (uint32_t)((((off & 3) << 2) | (((off >> 3) & 1) << 1)) << 4);
+    else return (uint32_t)(((((off >> 1) & 1) << 2) | (((off >> 3) & 1) << 1)) << 4);
+  }
+};
+
+// Moves tiles of ROWS rows from global memory to LDS with NT threads.  Row r of a tile is at base + offset(r), where
+// offset(r) = (r / g) * stride + (r % g) * inner (g rows lie `inner` apart, then `stride`): g = 1 for keys and values, the
+// heads of a group for queries.  DMA: rows of whole 16-byte chunks at 4-byte aligned addresses go straight to LDS;
+// otherwise they pass through registers (fetch before the computation on the tile before, put after it).
+template <typename T, int DP, int ROWS, int NT, bool DMA>
+struct TileLoader {
+  typedef Tile<T, DP> L;
+  static constexpr int kBytes = ROWS * L::kPitch;
+  static constexpr int kInstr = kBytes / 16 / NT;
+  static_assert(kBytes % (16 * NT) == 0, "a tile is a whole number of chunks per thread");
+  u32x4 held[DMA ? 1 : kInstr];
+
+  // rows_left: rows of the tile that exist (may be <= 0 or more than ROWS).  first: where the tile's first row lies in
+  // its group of g (0 when g == 1); base is the address of row -first.
+  __device__ inline void fetch(const T *base, int rows_left, uint32_t first, uint32_t g, uint32_t inv_g, uint32_t stride,
+                               uint32_t inner, int d, uint32_t lds_addr, int tid) {
+    if constexpr (DMA) {
+      const u32x4 rsrc = buffer_words(base, 0x7fffffffu);
+      const uint32_t wave_at = (uint32_t)__builtin_amdgcn_readfirstlane((tid & ~63) * 16);
+#pragma unroll
+      for (int q = 0; q < kInstr; ++q) {
+        const int slot = q * NT + tid;
+        uint32_t off;
+        const bool in = place(slot, rows_left, first, g, inv_g, stride, inner, d, &off);
+        lds_dma_b128(rsrc, lds_addr + wave_at + (uint32_t)(q * NT * 16), in ? off * (uint32_t)sizeof(T) : kOutOfRange);
+      }
+    } else {
+#pragma unroll
+      for (int q = 0; q < kInstr; ++q) {
+        uint32_t off;
+        const int slot = q * NT + tid;
+        const bool in = place(slot, rows_left, first, g, inv_g, stride, inner, d, &off);
+        const int c = (slot % L::kChunks) ^ L::swizzle(slot / L::kChunks);
+        held[q] = load_chunk(base + (in ? off : 0), in ? d - c * L::kPerChunk : 0);
+      }
+    }
+  }
+  __device__ inline void put(uint32_t lds_addr, int tid) {
+    if constexpr (!DMA) {
+#pragma unroll
+      for (int q = 0; q < kInstr; ++q) *lds_ptr<u32x4>(lds_addr + (uint32_t)((q * NT + tid) * 16)) = held[q];
+    }
+  }
+
+ private:
+  // Element offset of the chunk that belongs at position `slot` of the tile; false where nothing lies there.
+  __device__ static inline bool place(int slot, int rows_left, uint32_t first, uint32_t g, uint32_t inv_g, uint32_t stride,
+                                      uint32_t inner, int d, uint32_t *off) {
+    const int row = slot / L::kChunks, c = (slot % L::kChunks) ^ L::swizzle(row);
+    if (g == 1) {
+      *off = (uint32_t)row * stride + (uint32_t)(c * L::kPerChunk);
+    } else {
+      const uint32_t r = first + (uint32_t)row, t = (r * inv_g) >> 22;
+      *off = t * stride + (r - t * g) * inner + (uint32_t)(c * L::kPerChunk);
+    }
+    return row < rows_left && c * L::kPerChunk < d;
+  }
+};
+
+// ceil(2^22 / g): (r * inverse(g)) >> 22 == r / g for r * g < 2^22.  Rows inside a tile: r < 64 + g, g <= kMostGroup.
+inline uint32_t inverse(uint32_t g) { return ((1u << 22) + g - 1) / g; }
+constexpr uint32_t kMostGroup = 1024;
+
+// ---- small things ---------------------------------------------------------------------------------------------------
+
+// Maximum and sum over the two halves of a wavefront (lanes l and l ^ 32), the same bits in both.
+template <typename OP>
+__device__ inline float over_halves(float x, OP op) {
+  // the swap of a register's upper half with the lower half of its copy leaves the two halves in two registers
+  const uint32_t u = __builtin_bit_cast(uint32_t, x);
+  const auto r = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+  const uint32_t lo = r[0], hi = r[1];
+  return op(__builtin_bit_cast(float, lo), __builtin_bit_cast(float, hi));
+}
+__device__ inline float halves_max(float x) {
+  return over_halves(x, [](float a, float b) { return fmaxf(a, b); });
+}
+__device__ inline float halves_sum(float x) {
+  return over_halves(x, [](float a, float b) { return a + b; });
+}
+
+__device__ inline float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// Row of register i of a result block, without the 4 (lane / 32).
+__host__ __device__ constexpr int block_row(int i) { return (i & 3) + 8 * (i >> 2); }
+
+// Four consecutive elements p[0..3], of which the first `n` exist; `vec`: p is aligned to four elements.
+template <typename T, bool ACC>
+__device__ inline void store4(T *p, const float (&x)[4], int n, bool vec) {
+  if (vec && n >= 4) {
+    struct alignas(4 * sizeof(T)) Quad {
+      T v[4];
+    } q;
+    if constexpr (ACC) q = *reinterpret_cast<const Quad *>(p);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) q.v[e] = from_f32<T>(ACC ? to_f32(q.v[e]) + x[e] : x[e]);
+    *reinterpret_cast<Quad *>(p) = q;
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (e < n) p[e] = from_f32<T>(ACC ? to_f32(p[e]) + x[e] : x[e]);
+  }
+}
+
+// Where a workgroup's tile lies: tile `t` of sequence `e`, or (e.sample == kNoSequence) tile `t` of the rows behind the
+// last packed sequence.  `slot` counts the tiles of all sequences.
+//  * whole and padded samples: n tiles per step, the last tile of every sample first when `last_first` (with a causal mask
+//    the last rows see the most keys, so the long tiles start first);
+//  * packed: sequence i starts at slot floor(rows before it / size) + i, which leaves room for its ceil(rows / size)
+//    tiles; a slot that is left over has a tile past the end.
+constexpr uint32_t kNoSequence = 0xffffffffu;
+struct Place {
+  SequenceEntry e;
+  uint32_t t;
+};
+// rows_per: rows per token (g for queries, 1 for keys); tiles: tiles of a whole sample; by_keys: tiles of keys.
+__device__ inline Place find_place(const SequenceView &s, uint32_t slot, uint32_t tiles, uint32_t size, uint32_t rows_per,
+                                   bool by_keys, bool last_first) {
+  if (!s.packed) {
+    const uint32_t t = slot / s.n;
+    return {s.at(slot - t * s.n), last_first ? tiles - 1 - t : t};
+  }
+  const uint32_t total = by_keys ? s.k_total : s.q_total;
+  const uint32_t behind = (uint32_t)((uint64_t)total * rows_per / size) + s.n;
+  if (slot >= behind) return {{kNoSequence, 0, 0, 0, 0, 0, 0, 0}, slot - behind};
+  uint32_t lo = 0, hi = s.n;  // the last entry whose first slot is not behind `slot`
+  while (hi - lo > 1) {
+    const uint32_t mid = (lo + hi) / 2;
+    const uint32_t cum = by_keys ? s.entries[mid].k_cum : s.entries[mid].q_cum;
+    if ((uint32_t)((uint64_t)cum * rows_per / size) + mid <= slot) lo = mid;
+    else hi = mid;
+  }
+  const SequenceEntry e = s.entries[lo];
+  const uint32_t t = slot - ((uint32_t)((uint64_t)(by_keys ? e.k_cum : e.q_cum) * rows_per / size) + lo);
+  const uint32_t own = (uint32_t)(((uint64_t)(by_keys ? e.k_len : e.q_len) * rows_per + size - 1) / size);
+  return {e, last_first && t < own ? own - 1 - t : t};
+}
+// Slots that find_place can be asked for, per key head.
+inline uint64_t slots(const SequenceView &s, uint32_t size, uint32_t rows_per, bool by_keys) {
+  const uint64_t tokens = by_keys ? s.tk : s.tq, total = by_keys ? s.k_total : s.q_total;
+  if (!s.packed) return (uint64_t)s.n * ((tokens * rows_per + size - 1) / size);
+  return total * rows_per / size + s.n + ((tokens - total) * rows_per + size - 1) / size;
+}
+
+// ---- arguments ------------------------------------------------------------------------------------------------------
+
+struct Shape {
+  uint32_t d, hq, hk, g;      // head size, query heads, key heads, hq / hk
+  uint32_t inv_g;
+  uint32_t causal;
+  float scale_log2;           // scale * log2(e): scores are exponents of 2
+  float scale;
+};
+
+constexpr uint32_t kMostSize = 128;  // largest head size
+
+// Checks what the forward and the gradient calls have in common.
+inline int make_shape(uint32_t d, uint32_t hq, uint32_t hk, uint32_t tq, uint32_t tk, uint32_t bs, int causal, float scale,
+                      size_t item, Shape *out) {
+  PHIP_REQUIRE(d >= 1 && d <= kMostSize, "head sizes of 1 to %u are supported, got %u", kMostSize, d);
+  PHIP_REQUIRE(hq >= 1 && hk >= 1 && hq % hk == 0, "%u query heads cannot share %u key heads", hq, hk);
+  PHIP_REQUIRE(hq / hk <= kMostGroup, "more than %u query heads per key head", kMostGroup);
+  PHIP_REQUIRE(tq >= 1 && tk >= 1 && bs >= 1, "empty tensors");
+  PHIP_REQUIRE(tq <= 0x7fffffffu && tk <= 0x7fffffffu, "more than 2^31 - 1 tokens");
+  // offsets inside a tile of 64 rows are 32 bits wide
+  PHIP_REQUIRE((uint64_t)d * hq * item * 72 < 0x7fffffffu, "heads of %u x %u elements are too large", hq, d);
+  PHIP_REQUIRE(scale > 0.f && scale <= 1e30f, "the scale must be positive and at most 1e30");
+  *out = {d, hq, hk, hq / hk, inverse(hq / hk), causal != 0 ? 1u : 0u, scale * kLog2e, scale};
+  return PHIP_OK;
+}
+
+// Lets KERNEL use `bytes` of dynamic LDS (more than the default 64 KiB) on the context's device; done once per device.
+template <auto *KERNEL>
+int allow_lds(phip_ctx *ctx, int bytes) {
+  static std::atomic<uint64_t> done{0};
+  if (bytes <= 64 * 1024 || (ctx->device < 64 && ((done.load() >> ctx->device) & 1))) return PHIP_OK;
+  PHIP_HIP(hipFuncSetAttribute(reinterpret_cast<const void *>(KERNEL), hipFuncAttributeMaxDynamicSharedMemorySize, bytes));
+  if (ctx->device < 64) done.fetch_or(1ull << ctx->device);
+  return PHIP_OK;
+}
+
+// True when rows of d elements at all the pointers can be moved in 16-byte chunks that do not reach into the next row.
+inline bool rows_movable(uint32_t d, size_t item, std::initializer_list<const void *> ptrs) {
+  if (d * item % 16 != 0) return false;
+  for (const void *p : ptrs)
+    if (reinterpret_cast<uintptr_t>(p) % 16 != 0) return false;
+  return true;
+}
+
+}  // namespace attention
+}  // namespace phip
+
+#endif  // PHIP_ATTENTION_H_

@@ -338,6 +338,89 @@ class Tensor:
     __iadd__ = inplace_add
 
 
+class Sequences:
+    """Which tokens of a minibatch belong to which sequence (phip_sequences, include/phip.h): made once per batch
+    by HIP.new_sequences, read by every layer's rotary, norm_rotary and attention calls."""
+
+    def __init__(self, device, q_lens, k_lens, packed):
+        q_lens = [int(n) for n in q_lens]
+        k_lens = q_lens if k_lens is None else [int(n) for n in k_lens]
+        if not q_lens or len(q_lens) != len(k_lens):
+            raise Error("Invalid sequences: %d lengths of queries, %d of keys" % (len(q_lens), len(k_lens)))
+        if min(q_lens) < 0 or min(k_lens) < 0 or max(q_lens) >= 2 ** 31 or max(k_lens) >= 2 ** 31:
+            raise Error("Invalid length of a sequence")
+        self._device, self._ptr = device, ctypes.c_void_p()
+        self.q_lens, self.k_lens, self.packed = tuple(q_lens), tuple(k_lens), bool(packed)
+        aq, n = device._u32(q_lens)
+        ak, _ = device._u32(k_lens)
+        _lib.call("phip_sequences_create", device.ctx(), aq, ak, n, int(self.packed), ctypes.byref(self._ptr))
+
+    def __del__(self):
+        try:
+            if self._ptr:
+                _lib.lib().phip_sequences_destroy(self._ptr)
+        except Exception:
+            pass
+
+    def handle(self):
+        return self._ptr.value
+
+    def device(self):
+        return self._device
+
+
+class AttentionStats:
+    """What attention_fw leaves for attention_bw: the logarithm of each row's sum of exponentials, always fp32."""
+
+    def __init__(self, device, shape, handle):
+        self._device, self._shape, self._handle = device, shape, handle
+
+    def shape(self):
+        return self._shape
+
+    def device(self):
+        return self._device
+
+    def handle(self):
+        return self._handle.ptr
+
+    def to_vector(self):
+        out = np.empty(self._shape.size(), dtype=np.float32)
+        _lib.call("phip_memcpy_d2h", self._device.ctx(), out.ctypes.data, self._handle.ptr, out.nbytes)
+        return out
+
+
+def rotary_frequencies(pairs, base=10000.0, method="plain", factor=1.0, original_length=0, low=1.0, high=32.0):
+    """Frequencies of rotary positions and the amplitude that goes with them: (float32 array of `pairs`, float).
+
+    plain:  f[i] = base ** (-i / pairs).
+    linear: f / factor - positions squeezed into the length the model was trained on (Chen et al., "Extending
+            Context Window of Large Language Models via Positional Interpolation", 2023).
+    base:   the base grows so that the lowest frequency is divided by `factor` and the highest stays.
+    parts:  frequencies that turn fewer than `low` times within original_length are divided by factor, those that
+            turn more than `high` times stay, a linear ramp between; amplitude 0.1 ln(factor) + 1 (Peng et al.,
+            "YaRN: Efficient Context Window Extension of Large Language Models", 2023).
+    """
+    if pairs < 1 or not base > 1 or not factor >= 1:
+        raise Error("Invalid rotary frequencies. pairs: %d, base: %g, factor: %g" % (pairs, base, factor))
+    i = np.arange(pairs, dtype=np.float64)
+    f, amplitude = base ** (-i / pairs), 1.0
+    if method == "linear":
+        f = f / factor
+    elif method == "base":
+        if pairs > 1:
+            f = (base * factor ** (pairs / (pairs - 1.0))) ** (-i / pairs)
+    elif method == "parts":
+        if original_length < 1 or not high > low:
+            raise Error("Invalid scaling by parts. original_length: %d, low: %g, high: %g" % (original_length, low, high))
+        keep = np.clip((original_length * f / (2 * np.pi) - low) / (high - low), 0.0, 1.0)
+        f = f * (keep + (1 - keep) / factor)
+        amplitude = 0.1 * float(np.log(factor)) + 1.0
+    elif method != "plain":
+        raise Error("Unknown scaling of rotary frequencies: %r" % (method,))
+    return f.astype(np.float32), amplitude
+
+
 class DeviceType:
     # the reference's enum (primitiv/core/device.h:17-35) extended by one group
     GROUP_HIP = 0x00030000
@@ -990,6 +1073,141 @@ class HIP:
         _lib.call("phip_broadcast_fw_" + self._SUFFIX, self._ctx, x.handle(), y.mutable_handle(), base, size,
                   x.shape().size() // base)
         return y
+
+    # -- rotary positions, head norms and attention -----------------------------
+    # Tensors of [size, heads, tokens] x batch.  The reference has no counterpart; the names and the order of the
+    # arguments follow its conv2d_fw / conv2d_bw (operands, results, gradients of the results, parameters, gradients).
+    def new_sequences(self, q_lens, k_lens=None, packed=False):
+        """A list of sequences for the calls below (include/phip.h, phip_sequences_create)."""
+        return Sequences(self, q_lens, k_lens, packed)
+
+    def _seqs(self, seqs):
+        if seqs is None:
+            return None
+        if seqs.device() is not self:
+            raise Error("Device mismatched.")
+        return seqs.handle()
+
+    def _heads(self, name, tensors):
+        """Shapes of tensors of [size, heads, tokens] x batch."""
+        shapes = []
+        for t in tensors:
+            self._check_device(t)
+            shapes.append(t.shape())
+        if any(s.depth() > 3 for s in shapes):
+            raise Error("Invalid shapes at %s: %s" % (name, ", ".join(s.to_string() for s in shapes)))
+        return shapes
+
+    @staticmethod
+    def _mismatch(name, tensors):
+        raise Error("Shape mismatched at %s: %s" % (name, ", ".join(t.shape().to_string() for t in tensors)))
+
+    def _rotary_args(self, name, q, k, weights, freqs, interleaved, first, amplitude, seqs):
+        tensors = [q] if k is None else [q, k]
+        shapes = self._heads(name, tensors)
+        sq, sk = shapes[0], shapes[-1]
+        if sq[0] != sk[0] or sq[2] != sk[2] or sq.batch() != sk.batch():
+            self._mismatch(name, tensors)
+        for w in weights:
+            self._check_device(w)
+            if w.shape() != Shape([sq[0]]):
+                self._mismatch(name, tensors + list(weights))
+        freqs = np.ascontiguousarray(np.asarray(freqs, dtype=np.float32).reshape(-1))
+        if 2 * freqs.size > sq[0]:
+            raise Error("Invalid frequencies at %s: %d pairs in a head of %d elements" % (name, freqs.size, sq[0]))
+        if not -2 ** 31 <= int(first) < 2 ** 31:
+            raise Error("Invalid first position at %s: %d" % (name, first))
+        return (sq[0], sq[1], 0 if k is None else sk[1], sq[2], sq.batch(), self._seqs(seqs), int(first),
+                freqs.ctypes.data_as(ctypes.POINTER(ctypes.c_float)), freqs.size, int(bool(interleaved)),
+                float(amplitude)), freqs
+
+    @staticmethod
+    def _ptr(t):
+        return None if t is None else t.handle()
+
+    @staticmethod
+    def _mutable_ptr(t):
+        return None if t is None else t.mutable_handle()
+
+    def _rotary_bw_check(self, name, pairs):
+        """(operand, gradient) pairs of one shape each."""
+        for x, g in pairs:
+            if (x is None) != (g is None):
+                raise Error("Invalid arguments at %s: an operand without its gradient, or the other way round" % name)
+            if x is not None:
+                self._check_device(g)
+                if x.shape() != g.shape():
+                    self._mismatch(name, [x, g])
+
+    def rotary_fw(self, q, k, freqs, interleaved=False, first=0, amplitude=1.0, seqs=None):
+        """Queries and keys (or None) of the same tokens at their positions: a pair of tensors.  `freqs` as from
+        rotary_frequencies."""
+        args, held = self._rotary_args("rotary_fw", q, k, (), freqs, interleaved, first, amplitude, seqs)
+        yq, yk = self.new_raw_tensor(q.shape()), None if k is None else self.new_raw_tensor(k.shape())
+        _lib.call("phip_rotary_fw_" + self._SUFFIX, self._ctx, q.handle(), self._ptr(k), self._mutable_ptr(yq),
+                  self._mutable_ptr(yk), *args)
+        return yq, yk
+
+    def rotary_bw(self, gyq, gyk, freqs, interleaved, first, amplitude, seqs, gq, gk):
+        args, held = self._rotary_args("rotary_bw", gyq, gyk, (), freqs, interleaved, first, amplitude, seqs)
+        self._rotary_bw_check("rotary_bw", ((gyq, gq), (gyk, gk)))
+        pgq, pgk = self._mutable_ptr(gq), self._mutable_ptr(gk)
+        _lib.call("phip_rotary_bw_" + self._SUFFIX, self._ctx, gyq.handle(), self._ptr(gyk), pgq, pgk, *args)
+
+    def norm_rotary_fw(self, q, k, wq, wk, freqs, eps=1e-6, interleaved=False, first=0, amplitude=1.0, seqs=None):
+        """rotary_fw of the heads normalised to a root mean square of 1 and scaled by wq and wk."""
+        if (k is None) != (wk is None):
+            raise Error("Invalid arguments at norm_rotary_fw: keys without their weights, or the other way round")
+        args, held = self._rotary_args("norm_rotary_fw", q, k, (wq,) if k is None else (wq, wk), freqs, interleaved, first,
+                                       amplitude, seqs)
+        yq, yk = self.new_raw_tensor(q.shape()), None if k is None else self.new_raw_tensor(k.shape())
+        _lib.call("phip_norm_rotary_fw_" + self._SUFFIX, self._ctx, q.handle(), self._ptr(k), wq.handle(), self._ptr(wk),
+                  self._mutable_ptr(yq), self._mutable_ptr(yk), *args, float(eps))
+        return yq, yk
+
+    def norm_rotary_bw(self, q, k, wq, wk, gyq, gyk, freqs, eps, interleaved, first, amplitude, seqs, gq, gk, gwq, gwk):
+        if (k is None) != (wk is None) or (k is None) != (gyk is None):
+            raise Error("Invalid arguments at norm_rotary_bw: keys, their weights and the gradient of the result go together")
+        args, held = self._rotary_args("norm_rotary_bw", q, k, (wq,) if k is None else (wq, wk), freqs, interleaved, first,
+                                       amplitude, seqs)
+        self._rotary_bw_check("norm_rotary_bw", ((q, gyq), (k, gyk), (q, gq), (k, gk), (wq, gwq), (wk, gwk)))
+        pointers = [self._mutable_ptr(g) for g in (gq, gk, gwq, gwk)]
+        _lib.call("phip_norm_rotary_bw_" + self._SUFFIX, self._ctx, q.handle(), self._ptr(k), wq.handle(), self._ptr(wk),
+                  gyq.handle(), self._ptr(gyk), *pointers, *args, float(eps))
+
+    def _attention_args(self, name, q, k, v, causal, scale, seqs):
+        sq, sk, sv = self._heads(name, (q, k, v))
+        if sk != sv or sq[0] != sk[0] or sq.batch() != sk.batch() or sq[1] % sk[1] != 0:
+            self._mismatch(name, (q, k, v))
+        scale = 1.0 / float(np.sqrt(sq[0])) if scale is None else float(scale)
+        return (sq[0], sq[1], sk[1], sq[2], sk[2], sq.batch(), self._seqs(seqs), int(bool(causal)), scale)
+
+    def attention_fw(self, q, k, v, causal=True, scale=None, seqs=None, stats=False):
+        """softmax(scale q k^T) v; scale: None for 1 / sqrt(size).  With stats (needed by attention_bw): (y, stats)."""
+        args = self._attention_args("attention_fw", q, k, v, causal, scale, seqs)
+        y, kept = self.new_raw_tensor(q.shape()), None
+        if stats:
+            shape = Shape([q.shape()[1], q.shape()[2]], q.shape().batch())
+            ptr = ctypes.c_void_p()
+            _lib.call("phip_pool_alloc", self._ctx, 4 * shape.size(), ctypes.byref(ptr), None)
+            kept = AttentionStats(self, shape, _Handle(ptr.value, self._ctx_id, 0))
+        _lib.call("phip_attention_fw_" + self._SUFFIX, self._ctx, q.handle(), k.handle(), v.handle(), y.mutable_handle(),
+                  kept.handle() if stats else None, *args)
+        return (y, kept) if stats else y
+
+    def attention_bw(self, q, k, v, y, gy, stats, causal, scale, seqs, gq, gk, gv):
+        args = self._attention_args("attention_bw", q, k, v, causal, scale, seqs)
+        for x, t in ((q, y), (q, gy), (q, gq), (k, gk), (v, gv)):
+            self._check_device(t)
+            if x.shape() != t.shape():
+                self._mismatch("attention_bw", (q, k, v, y, gy, gq, gk, gv))
+        if stats.device() is not self:
+            raise Error("Device mismatched.")
+        if stats.shape() != Shape([q.shape()[1], q.shape()[2]], q.shape().batch()):
+            raise Error("Shape mismatched at attention_bw: stats of another call")
+        pointers = [self._mutable_ptr(g) for g in (gq, gk, gv)]
+        _lib.call("phip_attention_bw_" + self._SUFFIX, self._ctx, q.handle(), k.handle(), v.handle(), y.handle(),
+                  stats.handle(), gy.handle(), *pointers, *args)
 
     # -- random tensors ---------------------------------------------------------
     def _random(self, kind, shape, *params):

@@ -58,6 +58,10 @@ set(phip_SRCS
   ${PRIMITIV_HIP_BACKEND_DIR}/csrc/phip_gemm_h16_big.hip
   ${PRIMITIV_HIP_BACKEND_DIR}/csrc/phip_gemm_h16_skinny.hip
   ${PRIMITIV_HIP_BACKEND_DIR}/csrc/phip_matmul.hip
+  ${PRIMITIV_HIP_BACKEND_DIR}/csrc/phip_sequences.hip
+  ${PRIMITIV_HIP_BACKEND_DIR}/csrc/phip_rotary.hip
+  ${PRIMITIV_HIP_BACKEND_DIR}/csrc/phip_attention_fw.hip
+  ${PRIMITIV_HIP_BACKEND_DIR}/csrc/phip_attention_bw.hip
 )
 file(GLOB phip_HDRS "${PRIMITIV_HIP_BACKEND_DIR}/csrc/*.h" "${PRIMITIV_HIP_PHIP_INCLUDE_DIR}/phip.h")
 set(phip_FLAGS --offload-arch=gfx950 -O3 -std=c++17 -fPIC
