@@ -37,18 +37,25 @@ struct Rows {
   float m, l;           // l: this half's keys only
 };
 
-// One step: 32 KB keys whose rows lie in LDS.  lim: keys below it are visible to the lane's row.
-template <typename T, int DP, int KB>
-__device__ inline void step(Rows<DP> &st, const Frag<T> (&qf)[DP / 16], uint32_t k_at, uint32_t v_at, int key0, int lim,
-                            bool masked, float scale_log2, int lane) {
-  typedef Tile<T, DP> L;
+// One step over 32 KB keys whose rows lie in LDS, in three parts.  The scores:
+template <int KB>
+struct Scores {
   f32x16 s[KB];
+};
+template <typename T, int DP, int KB>
+__device__ inline void scores(Scores<KB> &sc, const Frag<T> (&qf)[DP / 16], uint32_t k_at) {
 #pragma unroll
   for (int kb = 0; kb < KB; ++kb) {
-    s[kb] = f32x16{};
+    sc.s[kb] = f32x16{};
 #pragma unroll
-    for (int c = 0; c < DP / 16; ++c) mma(s[kb], L::row_frag(k_at, kb, c), qf[c]);
+    for (int c = 0; c < DP / 16; ++c) mma(sc.s[kb], Tile<T, DP>::row_frag(k_at, kb, c), qf[c]);
   }
+}
+
+// The running softmax: the scores become exp(score - maximum).  lim: keys below it are visible to the lane's row.
+template <int DP, int KB>
+__device__ inline void softmax(Rows<DP> &st, Scores<KB> &sc, int key0, int lim, bool masked, float scale_log2, int lane) {
+  f32x16 (&s)[KB] = sc.s;
   if (masked) {
     const int first = key0 + 4 * (lane >> 5);
 #pragma unroll
@@ -81,13 +88,18 @@ __device__ inline void step(Rows<DP> &st, const Frag<T> (&qf)[DP / 16], uint32_t
       sum += s[kb][i];
     }
   st.l += sum;
+}
+
+// The product with the values.
+template <typename T, int DP, int KB>
+__device__ inline void values(Rows<DP> &st, const Scores<KB> &sc, uint32_t v_at) {
 #pragma unroll
   for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
-      const Frag<T> p = as_operand(s[kb], c, (Frag<T> *)nullptr);
+      const Frag<T> p = as_operand(sc.s[kb], c, (Frag<T> *)nullptr);
 #pragma unroll
-      for (int db = 0; db < DP / 32; ++db) mma(st.o[db], L::col_frag(v_at, 2 * kb + c, db), p);
+      for (int db = 0; db < DP / 32; ++db) mma(st.o[db], Tile<T, DP>::col_frag(v_at, 2 * kb + c, db), p);
     }
 }
 
@@ -188,15 +200,242 @@ __global__ __launch_bounds__(kThreads, 2) void rows_kernel(const FwArgs<T> a) {
     }
     __syncthreads();  // tile t is in LDS, and nobody reads the other stage any more
     if (t + 1 < n) fetch(t + 1);
-    if (t * KT < w_keys)
-      step<T, DP, KT / 32>(st, qf, stage + row_at, stage + kTile + col_at, t * KT, lim, (t + 1) * KT > w_all,
-                           sh.scale_log2, lane);
+    if (t * KT < w_keys) {
+      Scores<KT / 32> sc;
+      scores<T, DP, KT / 32>(sc, qf, stage + row_at);
+      softmax<DP, KT / 32>(st, sc, t * KT, lim, (t + 1) * KT > w_all, sh.scale_log2, lane);
+      values<T, DP, KT / 32>(st, sc, stage + kTile + col_at);
+    }
   }
 
   const float l = halves_sum(st.l);
   if (!exists) return;
   store_row<T, DP>(a.y + row * sh.d, st.o, 1.f / l, valid && l != 0.f, sh.d, a.vec_y != 0, lane);
   if (a.stats != nullptr && lane < 32) a.stats[row] = !valid || l == 0.f ? -INFINITY : fmaf(st.m, sh.scale, logf(l));
+}
+
+// Few rows (a new token per sequence against its cache, short prompts): what takes the time is reading the keys and values
+// once, so a workgroup takes 32 rows and a range of the keys, its four wavefronts take blocks of 32 keys in turn, and the
+// partial results (maximum, sum, unnormalised rows) meet in LDS, and between the ranges of a tile in memory: the workgroup
+// that finishes last of a tile's ranges merges them in order.
+//
+// Every wavefront has a ring of LDS tiles of its own and waits for nobody else: K and V blocks alternate in it, and the
+// block `kRing` positions ahead is ordered as soon as a block has been used, so that up to three quarters of 128 KiB are on
+// their way to every CU.
+template <typename T, int DP>
+constexpr int kStages = 32 * Tile<T, DP>::kPitch <= 8192 ? 2 : 1;  // pairs of K and V: 128 KiB of LDS at most
+template <typename T, int DP>
+constexpr int kFewLds = std::max(kWaves * 2 * kStages<T, DP> * 32 * Tile<T, DP>::kPitch, kWaves * (DP * 33 + 64) * 4);
+
+// Device-scope accesses for what travels between workgroups, which may sit behind different L2 caches.
+__device__ inline void store_shared(float *p, float x) {
+  __hip_atomic_store(p, x, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ inline float load_shared(const float *p) {
+  return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+
+// True in the workgroup that is the last of `count` to get here.  Each lane waits until memory has acknowledged its own
+// stores, the barrier puts all of them before thread 0's ticket, and the ticket is a device-scope atomic on one address,
+// so whoever draws the last one finds what the others stored.  The counter is left zeroed for the next launch.
+__device__ inline bool last_of_tile(uint32_t *ticket, uint32_t count, uint32_t *flag) {
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    const uint32_t drawn = __hip_atomic_fetch_add(ticket, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    const bool last = drawn == count - 1u;
+    if (last) __hip_atomic_store(ticket, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    *flag = last ? 1u : 0u;
+  }
+  __syncthreads();
+  return *flag != 0;
+}
+
+template <typename T, int DP, bool DMA>
+__global__ __launch_bounds__(kThreads, 1) void few_kernel(const FwArgs<T> a) {
+  constexpr int BM = 32, S = kStages<T, DP>;
+  typedef Tile<T, DP> L;
+  typedef TileLoader<T, DP, 32, 64, DMA> Loader;
+  constexpr uint32_t kTile = (uint32_t)Loader::kBytes;
+  extern __shared__ __attribute__((aligned(1024))) unsigned char lds[];
+  __shared__ uint32_t flag;
+  const uint32_t lds0 = (uint32_t)(size_t)(__attribute__((address_space(3))) unsigned char *)lds;
+
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const Shape &sh = a.s;
+  const uint32_t head = blockIdx.x % sh.hk, range = blockIdx.x / sh.hk % a.splits, slot = blockIdx.x / sh.hk / a.splits;
+  const Place at = find_place(a.seq, slot, a.tiles, BM, sh.g, false, sh.causal != 0);
+  const SequenceEntry &e = at.e;
+  const bool behind = e.sample == kNoSequence;
+  const uint32_t token0 = behind ? a.seq.q_total : e.q_start;
+  const size_t sample = behind ? 0 : e.sample;
+  const uint32_t tokens = behind ? a.seq.tq - a.seq.q_total : a.seq.packed ? e.q_len : a.seq.tq;
+  const int64_t r0 = (int64_t)at.t * BM, rows = min((int64_t)tokens * sh.g - r0, (int64_t)BM);
+  if (rows <= 0) return;
+  const int lq = behind ? 0 : (int)e.q_len, lk = (int)e.k_len;
+
+  const int64_t r = r0 + (lane & 31);
+  const uint32_t tok = (uint32_t)(r / sh.g);
+  const bool exists = tok < tokens, valid = exists && (int)tok < lq;
+  const int lim = !valid ? 0 : sh.causal ? min(lk, max(0, (int)tok + lk - lq + 1)) : lk;
+  const int64_t last = min((int64_t)lq * sh.g, r0 + BM) - 1;
+  const int keys = last < r0 ? 0 : sh.causal ? min(lk, max(0, (int)(last / sh.g) + lk - lq + 1)) : lk;
+  const int all = last < r0 || last < r0 + BM - 1 ? 0 : sh.causal ? min(lk, max(0, (int)(r0 / sh.g) + lk - lq + 1)) : lk;
+  const uint32_t ranges = max(1u, ((uint32_t)keys + a.chunk - 1) / a.chunk);
+  if (range >= ranges) return;
+  const int from = (int)(range * a.chunk), to = min(keys, from + (int)a.chunk);
+
+  auto row_of = [&](int64_t rr) {
+    return (sample * a.seq.tq + token0 + (uint32_t)(rr / sh.g)) * sh.hq + head * sh.g + (uint32_t)(rr % sh.g);
+  };
+  Frag<T> qf[DP / 16];
+  {
+    const size_t row = row_of(exists ? r : r0);
+#pragma unroll
+    for (int c = 0; c < DP / 16; ++c)
+      qf[c] = load_frag(a.q + row * sh.d, valid, 16 * c + 8 * (lane >> 5), (int)sh.d, (Frag<T> *)nullptr);
+  }
+  Rows<DP> st;
+  reset(st);
+  const uint32_t stride = sh.hk * sh.d;
+  const T *kp = a.k + ((sample * a.seq.tk + e.k_start) * sh.hk + head) * (size_t)sh.d;
+  const T *vp = a.v + ((sample * a.seq.tk + e.k_start) * sh.hk + head) * (size_t)sh.d;
+  const uint32_t ring = lds0 + (uint32_t)wave * (2 * S * kTile);
+  const uint32_t row_at = L::row_lane(lane), col_at = L::col_lane(lane);
+  Loader lk_, lv_;
+  auto fetch_k = [&](int key, int s) {
+    lk_.fetch(kp + (size_t)min(key, to) * stride, to - key, 0, 1, 0, stride, 0, (int)sh.d, ring + (uint32_t)s * 2 * kTile, lane);
+  };
+  auto fetch_v = [&](int key, int s) {
+    lv_.fetch(vp + (size_t)min(key, to) * stride, to - key, 0, 1, 0, stride, 0, (int)sh.d, ring + (uint32_t)s * 2 * kTile + kTile, lane);
+  };
+  constexpr int kStep = 32 * kWaves;
+  int key = from + 32 * wave;
+  if constexpr (DMA) {
+    // blocks past the end are ordered too (they read nothing and write zeros), so that the waits count the same
+    constexpr int kInFlight = (2 * S - 1) * Loader::kInstr;
+#pragma unroll
+    for (int s = 0; s < S; ++s) {
+      fetch_k(key + s * kStep, s);
+      fetch_v(key + s * kStep, s);
+    }
+    for (int s = 0; key < to; key += kStep, s = s + 1 == S ? 0 : s + 1) {
+      const uint32_t stage = ring + (uint32_t)s * 2 * kTile;
+      wait_loads<kInFlight>();
+      Scores<1> sc;
+      scores<T, DP, 1>(sc, qf, stage + row_at);
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the block's reads are done before its place is filled again
+      fetch_k(key + S * kStep, s);
+      softmax<DP, 1>(st, sc, key, lim, key + 32 > all, sh.scale_log2, lane);
+      wait_loads<kInFlight>();
+      values<T, DP, 1>(st, sc, stage + kTile + col_at);
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      fetch_v(key + S * kStep, s);
+    }
+    wait_loads<0>();  // nothing may land in the LDS that is used for something else below
+  } else {
+    if (key < to) {
+      fetch_k(key, 0);
+      fetch_v(key, 0);
+    }
+    for (; key < to; key += kStep) {
+      lk_.put(ring, lane);
+      lv_.put(ring + kTile, lane);
+      if (key + kStep < to) {
+        fetch_k(key + kStep, 0);
+        fetch_v(key + kStep, 0);
+      }
+      Scores<1> sc;
+      scores<T, DP, 1>(sc, qf, ring + row_at);
+      softmax<DP, 1>(st, sc, key, lim, key + 32 > all, sh.scale_log2, lane);
+      values<T, DP, 1>(st, sc, ring + kTile + col_at);
+    }
+  }
+
+  // the wavefronts' results: per wavefront DP columns of 33 floats (rows across), then 32 maxima and 32 sums
+  __syncthreads();
+  float *const area = reinterpret_cast<float *>(lds);
+  constexpr int kPer = DP * 33 + 64;
+  {
+    float *mine = area + wave * kPer;
+#pragma unroll
+    for (int db = 0; db < DP / 32; ++db)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) mine[(32 * db + block_row(i) + 4 * (lane >> 5)) * 33 + (lane & 31)] = st.o[db][i];
+    const float l = halves_sum(st.l);
+    if (lane < 32) {
+      mine[DP * 33 + lane] = valid ? st.m : -INFINITY;
+      mine[DP * 33 + 32 + lane] = valid ? l : 0.f;
+    }
+  }
+  __syncthreads();
+  const bool whole = ranges == 1;
+  const uint32_t tile = slot * sh.hk + head;
+  float *const part = a.partial + ((size_t)tile * a.splits + range) * (size_t)(BM * (DP + 2));
+  auto finish = [&](int row, uint32_t dd, float o, float m, float l) {
+    const size_t at_row = row_of(r0 + row);
+    a.y[at_row * sh.d + dd] = from_f32<T>(l == 0.f ? 0.f : o / l);
+    if (dd == 0 && a.stats != nullptr) a.stats[at_row] = l == 0.f ? -INFINITY : fmaf(m, sh.scale, logf(l));
+  };
+  for (uint32_t i = tid; i < (uint32_t)rows * DP; i += kThreads) {
+    const int row = (int)(i / DP);
+    const uint32_t dd = i % DP;
+    float m = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) m = fmaxf(m, area[w * kPer + DP * 33 + row]);
+    const float base = m == -INFINITY ? 0.f : m * sh.scale_log2;
+    float l = 0.f, o = 0.f;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) {
+      const float *his = area + w * kPer;
+      const float lw = his[DP * 33 + 32 + row];
+      if (lw == 0.f) continue;  // it has seen no key of this row
+      const float f = exp2_fast(fmaf(his[DP * 33 + row], sh.scale_log2, -base));
+      l = fmaf(lw, f, l);
+      o = fmaf(his[dd * 33 + row], f, o);
+    }
+    if (whole) {
+      if (dd < sh.d) finish(row, dd, o, m, l);
+    } else {
+      store_shared(part + row * (DP + 2) + dd, o);
+      if (dd < 2) store_shared(part + row * (DP + 2) + DP + dd, dd == 0 ? m : l);
+    }
+  }
+  if (whole || !last_of_tile(a.tickets + tile, ranges, &flag)) return;
+  // The last of the tile: each thread has one element of a row at a time and takes the ranges 16 at a time, all their
+  // loads in flight together.
+  const float *const all_parts = a.partial + (size_t)tile * a.splits * (size_t)(BM * (DP + 2));
+  for (uint32_t i = tid; i < (uint32_t)rows * DP; i += kThreads) {
+    const int row = (int)(i / DP);
+    const uint32_t dd = i % DP;
+    float m = -INFINITY, l = 0.f, o = 0.f;
+    for (uint32_t p0 = 0; p0 < ranges; p0 += 16) {
+      float pm[16], pl[16], po[16];
+#pragma unroll
+      for (uint32_t u = 0; u < 16; ++u) {
+        const float *p = all_parts + (size_t)min(p0 + u, ranges - 1) * (BM * (DP + 2)) + row * (DP + 2);
+        pm[u] = load_shared(p + DP);
+        pl[u] = load_shared(p + DP + 1);
+        po[u] = load_shared(p + dd);
+      }
+      float top = m;
+#pragma unroll
+      for (uint32_t u = 0; u < 16; ++u) top = fmaxf(top, pm[u]);
+      const float base = top == -INFINITY ? 0.f : top * sh.scale_log2;
+      const float f = l == 0.f ? 0.f : exp2_fast(fmaf(m, sh.scale_log2, -base));
+      l *= f;
+      o *= f;
+      m = top;
+#pragma unroll
+      for (uint32_t u = 0; u < 16; ++u) {
+        const float fu = p0 + u >= ranges || pl[u] == 0.f ? 0.f : exp2_fast(fmaf(pm[u], sh.scale_log2, -base));
+        if (fu == 0.f) continue;
+        l = fmaf(pl[u], fu, l);
+        o = fmaf(po[u], fu, o);
+      }
+    }
+    if (dd < sh.d) finish(row, dd, o, m, l);
+  }
 }
 
 template <typename T, int DP, bool DMA>
@@ -213,8 +452,48 @@ int launch_rows(phip_ctx *ctx, FwArgs<T> a) {
   return PHIP_OK;
 }
 
+// Keys per range of the kernel for few rows.  One workgroup fits on a CU (its ring of tiles), so the time is about the
+// keys of a range times the rounds that the ranges take on the chip: the shortest range that fills it once, or, when
+// there are more tiles than that, ranges of a quarter of the average, which even out different lengths.
+uint32_t few_chunk(phip_ctx *ctx, const SequenceView &view, const phip_sequences *seqs, const Shape &s, uint64_t tiles) {
+  const uint64_t cus = (uint64_t)ctx->prop.multiProcessorCount;
+  const uint64_t most = seqs != nullptr ? seqs->max_k : view.tk;
+  if (tiles > (uint64_t)kTicketSlots) return (uint32_t)most + 1;
+  const uint64_t keys = (seqs != nullptr ? seqs->k_sum : (uint64_t)view.n * view.tk) * s.hk;
+  uint64_t chunk = (keys + cus - 1) / cus;
+  if (chunk < 256) chunk = 256;
+  return (uint32_t)std::min<uint64_t>((chunk + 127) / 128 * 128, 1u << 30);
+}
+
+template <typename T, int DP, bool DMA>
+int launch_few(phip_ctx *ctx, FwArgs<T> a, const phip_sequences *seqs) {
+  constexpr int lds = kFewLds<T, DP>;
+  const int rc = allow_lds<few_kernel<T, DP, DMA>>(ctx, lds);
+  if (rc != PHIP_OK) return rc;
+  a.tiles = (uint32_t)(((uint64_t)a.seq.tq * a.s.g + 31) / 32);
+  const uint64_t tiles = slots(a.seq, 32, a.s.g, false) * a.s.hk;
+  a.chunk = few_chunk(ctx, a.seq, seqs, a.s, tiles);
+  const uint32_t most = seqs != nullptr ? seqs->max_k : a.seq.tk;
+  a.splits = most <= a.chunk ? 1 : (most + a.chunk - 1) / a.chunk;
+  PHIP_REQUIRE(tiles * a.splits < 0x7fffffffu, "too many rows");
+  void *partial = nullptr;
+  if (a.splits > 1) {
+    const int rc2 = phip_pool_alloc(ctx, (size_t)tiles * a.splits * 32 * (DP + 2) * sizeof(float), &partial, nullptr);
+    if (rc2 != PHIP_OK) return rc2;
+    a.partial = static_cast<float *>(partial);
+    a.tickets = tile_tickets(ctx);
+  }
+  hipLaunchKernelGGL((few_kernel<T, DP, DMA>), dim3((uint32_t)(tiles * a.splits)), dim3(kThreads), lds, ctx->stream, a);
+  const hipError_t e = hipGetLastError();
+  if (partial != nullptr) phip_pool_free(ctx, partial);
+  if (e != hipSuccess) return fail(PHIP_ERR_RUNTIME, "launching the attention kernel failed: %s", hipGetErrorString(e));
+  return PHIP_OK;
+}
+
 template <typename T, int DP>
-int launch(phip_ctx *ctx, const FwArgs<T> &a, bool dma) {
+int launch(phip_ctx *ctx, const FwArgs<T> &a, const phip_sequences *seqs, bool dma) {
+  const uint32_t most = seqs != nullptr ? seqs->max_q : a.seq.tq;
+  if ((uint64_t)most * a.s.g <= 32) return dma ? launch_few<T, DP, true>(ctx, a, seqs) : launch_few<T, DP, false>(ctx, a, seqs);
   return dma ? launch_rows<T, DP, true>(ctx, a) : launch_rows<T, DP, false>(ctx, a);
 }
 
@@ -239,10 +518,10 @@ int forward(phip_ctx *ctx, const T *q, const T *k, const T *v, T *y, float *stat
   a.vec_y = d % 4 == 0 && reinterpret_cast<uintptr_t>(y) % (4 * sizeof(T)) == 0;
   const bool dma = rows_movable(d, sizeof(T), {k, v});
   switch ((d + 31) / 32) {
-    case 1: return launch<T, 32>(ctx, a, dma);
-    case 2: return launch<T, 64>(ctx, a, dma);
-    case 3: return launch<T, 96>(ctx, a, dma);
-    default: return launch<T, 128>(ctx, a, dma);
+    case 1: return launch<T, 32>(ctx, a, seqs, dma);
+    case 2: return launch<T, 64>(ctx, a, seqs, dma);
+    case 3: return launch<T, 96>(ctx, a, seqs, dma);
+    default: return launch<T, 128>(ctx, a, seqs, dma);
   }
 }
 

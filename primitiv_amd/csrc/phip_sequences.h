@@ -46,7 +46,8 @@ struct phip_sequences {
   uint32_t n = 0;
   bool packed = false;
   uint32_t max_q = 0, max_k = 0;
-  uint32_t q_total = 0, k_total = 0;
+  uint32_t q_total = 0, k_total = 0;  // packed
+  uint64_t k_sum = 0;                 // keys of all sequences
 };
 
 namespace phip {

@@ -66,6 +66,7 @@ int create(phip_ctx *ctx, const uint32_t *q_lens, const uint32_t *k_lens, uint32
   s->max_k = max_k;
   s->q_total = packed ? (uint32_t)q_at : 0;
   s->k_total = packed ? (uint32_t)k_at : 0;
+  s->k_sum = k_at;
   const int rc = phip_pool_alloc(ctx, (sizeof(SequenceEntry) + sizeof(SequencePlace)) * (size_t)n, &s->block, nullptr);
   if (rc != PHIP_OK) {
     delete s;

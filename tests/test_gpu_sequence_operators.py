@@ -65,6 +65,9 @@ ATTENTION = {
     "padded_not_causal": (32, 3, 3, 50, 70, 4, (50, 7, 0, 31), (70, 0, 5, 64), False, False),
     "cache": (128, 8, 2, 1, 300, 6, (1, 1, 1, 1, 0, 1), (300, 1, 63, 64, 9, 65), False, True),
     "cache_new_tokens": (96, 6, 2, 5, 257, 3, (5, 5, 3), (257, 5, 128), False, True),
+    "long_cache": (64, 4, 1, 2, 5000, 3, (2, 1, 2), (5000, 1500, 2), False, True),
+    "long_cache_odd_size": (33, 3, 3, 1, 2100, 1, None, None, False, False),
+    "packed_tokens": (128, 8, 2, 9, 1200, 1, (1, 3, 0, 4), (700, 3, 5, 450), True, True),
     "packed": (64, 4, 2, 200, 200, 1, (70, 1, 0, 64, 65), None, True, True),
     "packed_tail": (128, 4, 4, 160, 170, 1, (33, 1, 64), (40, 0, 97), True, True),
     "packed_many": (32, 2, 1, 300, 300, 1, (1,) * 40 + (0, 3, 130, 2), None, True, False),
