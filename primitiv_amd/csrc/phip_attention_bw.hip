@@ -166,7 +166,7 @@ template <typename T>
 constexpr int kRows = sizeof(T) == 2 ? 64 : 32;
 
 template <typename T, int DP, bool DMA>
-__global__ __launch_bounds__(kThreads, 1) void keys_kernel(const BwArgs<T> a) {
+__global__ __launch_bounds__(kThreads, sizeof(T) == 2 && DMA ? 2 : 1) void keys_kernel(const BwArgs<T> a) {
   constexpr int QT = kRows<T>, BN = 32 * kWaves;
   typedef Tile<T, DP> L;
   typedef TileLoader<T, DP, QT, kThreads, DMA> Loader;
@@ -247,35 +247,47 @@ __global__ __launch_bounds__(kThreads, 1) void keys_kernel(const BwArgs<T> a) {
     if (r + QT < rows) fetch(r + QT, s ^ 1);
     if (r + QT <= w_first) continue;  // none of these rows sees a key of the wavefront
     const bool masked = r < w_all;
-#pragma unroll
+#pragma unroll 1
     for (int qb = 0; qb < QT / 32; ++qb) {
-      f32x16 p = f32x16{}, dp = f32x16{};
-#pragma unroll
-      for (int c = 0; c < DP / 16; ++c) mma(p, L::row_frag(stage + row_at, qb, c), kf[c]);
-#pragma unroll
-      for (int c = 0; c < DP / 16; ++c) mma(dp, L::row_frag(stage + kTile + row_at, qb, c), vf[c]);
+      const uint32_t q_at = stage + (uint32_t)(qb * 32 * L::kPitch), g_at = q_at + kTile;
+      const uint32_t in = values + (uint32_t)((32 * qb + 4 * (lane >> 5)) * 4);
       const int hidden = (int)max((int64_t)0, min((int64_t)QT, my_first - r)) - 32 * qb - 4 * (lane >> 5);
+      f32x16 p = f32x16{};
+#pragma unroll
+      for (int c = 0; c < DP / 16; ++c) mma(p, L::row_frag(q_at + row_at, 0, c), kf[c]);
 #pragma unroll
       for (int i4 = 0; i4 < 4; ++i4) {
-        const uint32_t in = values + (uint32_t)((32 * qb + 8 * i4 + 4 * (lane >> 5)) * 4);
-        const f32x4 base = *lds_ptr<f32x4>(in), delta = *lds_ptr<f32x4>(in + QT * 4);
+        const f32x4 base = *lds_ptr<f32x4>(in + 32 * i4);
 #pragma unroll
         for (int e4 = 0; e4 < 4; ++e4) {
           const int i = 4 * i4 + e4;
-          float x = exp2_fast(fmaf(p[i], sh.scale_log2, -base[e4]));
-          if (masked && block_row(i) < hidden) x = 0.f;
-          p[i] = x;
-          dp[i] = x == 0.f ? 0.f : x * (dp[i] - delta[e4]);
+          p[i] = exp2_fast(fmaf(p[i], sh.scale_log2, -base[e4]));
+          if (masked && block_row(i) < hidden) p[i] = 0.f;
         }
       }
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
-        const Frag<T> pf = as_operand(p, c, (Frag<T> *)nullptr), ds = as_operand(dp, c, (Frag<T> *)nullptr);
+        const Frag<T> pf = as_operand(p, c, (Frag<T> *)nullptr);
 #pragma unroll
-        for (int db = 0; db < DP / 32; ++db) {
-          mma(gv[db], L::col_frag(stage + kTile + col_at, 2 * qb + c, db), pf);
-          mma(gk[db], L::col_frag(stage + col_at, 2 * qb + c, db), ds);
+        for (int db = 0; db < DP / 32; ++db) mma(gv[db], L::col_frag(g_at + col_at, c, db), pf);
+      }
+      f32x16 dp = f32x16{};
+#pragma unroll
+      for (int c = 0; c < DP / 16; ++c) mma(dp, L::row_frag(g_at + row_at, 0, c), vf[c]);
+#pragma unroll
+      for (int i4 = 0; i4 < 4; ++i4) {
+        const f32x4 delta = *lds_ptr<f32x4>(in + QT * 4 + 32 * i4);
+#pragma unroll
+        for (int e4 = 0; e4 < 4; ++e4) {
+          const int i = 4 * i4 + e4;
+          dp[i] = p[i] == 0.f ? 0.f : p[i] * (dp[i] - delta[e4]);
         }
+      }
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        const Frag<T> ds = as_operand(dp, c, (Frag<T> *)nullptr);
+#pragma unroll
+        for (int db = 0; db < DP / 32; ++db) mma(gk[db], L::col_frag(q_at + col_at, c, db), ds);
       }
     }
   }
