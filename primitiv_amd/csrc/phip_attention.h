@@ -41,6 +41,17 @@ __device__ inline __attribute__((address_space(3))) T *lds_ptr(uint32_t addr) {
   return (__attribute__((address_space(3))) T *)(size_t)addr;
 }
 
+// ---- arguments ---------------------------------------------------------------------------------------------------
+
+struct Shape {
+  uint32_t d, hq, hk, g;      // head size, query heads, key heads, hq / hk
+  uint32_t inv_g;
+  uint32_t causal;
+  float scale_log2;           // scale * log2(e): scores are exponents of 2
+  float scale;
+  uint32_t whole;             // rows are whole 16-byte chunks at addresses that are multiples of 16
+};
+
 // ---- fragments ------------------------------------------------------------------------------------------------------
 
 template <typename T>
@@ -107,39 +118,88 @@ struct alignas(sizeof(T)) Chunk {  // 16 bytes at any address that suits the ele
   T v[16 / sizeof(T)];
 };
 
-// `n` valid elements (at most one 16-byte chunk) at p, zeros behind them.
-template <typename T>
-__device__ inline u32x4 load_chunk(const T *p, int n) {
-  constexpr int N = 16 / sizeof(T);
-  u32x4 r = {0, 0, 0, 0};
-  if (n >= N) {
-    __builtin_memcpy(&r, reinterpret_cast<const Chunk<T> *>(p), 16);
-  } else if (n > 0) {
+// 16 bytes of a row of d elements from element c0 on (a multiple of 16 bytes), zeros behind the row's end; all zeros unless
+// `in`, which says that the row exists and c0 < d.
+// WHOLE: d is a whole number of 16-byte chunks and the rows are aligned to them.  Otherwise the last chunk is read so that
+// it ends with the row, and shifted into place by the same amount in all lanes: nothing waits for a load in either case, so
+// that all of a lane's loads are in flight together.  Only rows shorter than one chunk (TINY: they may be) go element by
+// element.  A lane
+// without a part of the row then loads nothing: 16-byte loads at addresses that are no multiple of 16 cost their time per
+// lane (fp32 heads of 65: 39 against 51 us with every lane loading).
+template <bool WHOLE, bool TINY, typename T>
+__device__ inline u32x4 load_part(const T *row, bool in, int c0, int d) {
+  constexpr int N = 16 / (int)sizeof(T);
+  u32x4 x = {0, 0, 0, 0};
+  if constexpr (WHOLE) {
+    x = *reinterpret_cast<const u32x4 *>(row + (in ? c0 : 0));
+  } else if (!TINY || d >= N) {
+    if (in) __builtin_memcpy(&x, reinterpret_cast<const Chunk<T> *>(row + min(c0, d - N)), 16);
+    const int missing = d % N;
+    if (missing != 0) {
+      const uint32_t bytes = (uint32_t)(N - missing) * (uint32_t)sizeof(T);
+      u32x4 y = x;
+      if (bytes & 4) y = u32x4{y[1], y[2], y[3], 0};
+      if (bytes & 8) y = u32x4{y[2], y[3], 0, 0};
+      if (bytes & 2) y = u32x4{y[0] >> 16 | y[1] << 16, y[1] >> 16 | y[2] << 16, y[2] >> 16 | y[3] << 16, y[3] >> 16};
+      x = c0 > d - N ? y : x;
+    }
+  } else if (in) {
     T e[N] = {};
 #pragma unroll
     for (int i = 0; i < N - 1; ++i)
-      if (i < n) e[i] = p[i];
-    __builtin_memcpy(&r, e, 16);
+      if (c0 + i < d) e[i] = row[c0 + i];
+    __builtin_memcpy(&x, e, 16);
   }
-  return r;
+  return in ? x : u32x4{0, 0, 0, 0};
 }
 
-// A lane's 8 elements d0 .. d0 + 7 of a row of `d` elements, zeros behind the row's end or for an absent row.
-template <typename T>
-__device__ inline Frag16<T> load_frag(const T *row, bool valid, int d0, int d, Frag16<T> *) {
-  return {load_chunk(row + (valid ? d0 : 0), valid ? d - d0 : 0)};
-}
-__device__ inline f32x8 load_frag(const float *row, bool valid, int d0, int d, f32x8 *) {
-  const u32x4 lo = load_chunk(row + (valid ? d0 : 0), valid ? d - d0 : 0);
-  const u32x4 hi = load_chunk(row + (valid && d - d0 > 4 ? d0 + 4 : 0), valid ? d - d0 - 4 : 0);
-  f32x8 f;
+// A lane's 8 elements d0 .. d0 + 7 of a row, zeros behind the row's end or for a row that is not `valid` (the address of an
+// existing row is needed all the same).
+template <bool WHOLE, bool TINY, typename T>
+__device__ inline Frag<T> load_frag(const T *row, bool valid, int d0, int d) {
+  if constexpr (sizeof(T) == 2) {
+    return {load_part<WHOLE, TINY>(row, valid && d0 < d, d0, d)};
+  } else {
+    const u32x4 lo = load_part<WHOLE, TINY>(row, valid && d0 < d, d0, d), hi = load_part<WHOLE, TINY>(row, valid && d0 + 4 < d, d0 + 4, d);
+    f32x8 f;
 #pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    const uint32_t l = lo[e], h = hi[e];  // a bit cast of a vector's element itself takes the first one
-    f[e] = __builtin_bit_cast(float, l);
-    f[e + 4] = __builtin_bit_cast(float, h);
+    for (int e = 0; e < 4; ++e) {
+      const uint32_t l = lo[e], h = hi[e];  // a bit cast of a vector's element itself takes the first one
+      f[e] = __builtin_bit_cast(float, l);
+      f[e + 4] = __builtin_bit_cast(float, h);
+    }
+    return f;
   }
-  return f;
+}
+
+// All of a lane's parts of a row: 16 c + 8 (lane / 32) + 0 .. 7.
+template <typename T, int NC>
+__device__ inline void load_row(Frag<T> (&f)[NC], const T *row, bool valid, const Shape &s, int lane) {
+  if (s.whole) {
+#pragma unroll
+    for (int c = 0; c < NC; ++c) f[c] = load_frag<true, false>(row, valid, 16 * c + 8 * (lane >> 5), (int)s.d);
+  } else {
+#pragma unroll
+    for (int c = 0; c < NC; ++c) f[c] = load_frag<false, NC == 2>(row, valid, 16 * c + 8 * (lane >> 5), (int)s.d);
+  }
+}
+
+// The compiler has waited for these loads when it gets here: a loop that counts its own loads behind this would otherwise
+// wait for all of them in every round, because the first one may find these still on their way.
+template <typename F, int N>
+__device__ inline void arrived(const F (&f)[N]) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    if constexpr (sizeof(F) == 16) {
+      asm volatile("" ::"v"(f[i].v) : "memory");
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float x = f[i][j];
+        asm volatile("" ::"v"(x) : "memory");
+      }
+    }
+  }
 }
 
 template <typename T>
@@ -154,7 +214,8 @@ __device__ inline u32x4 buffer_words(const void *p, uint32_t bytes) {
   const uint64_t a = reinterpret_cast<uint64_t>(p);
   // the address is the same in all lanes, which the compiler cannot always see
   u32x4 r = {(uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)a),
-             (uint32_t)__builtin_amdgcn_readfirstlane((int)((uint32_t)(a >> 32) & 0xffffu)), bytes, 0x00020000u};
+             (uint32_t)__builtin_amdgcn_readfirstlane((int)((uint32_t)(a >> 32) & 0xffffu)),
+             (uint32_t)__builtin_amdgcn_readfirstlane((int)bytes), 0x00020000u};
   return r;
 }
 
@@ -165,7 +226,14 @@ __device__ inline u32x4 buffer_words(const void *p, uint32_t bytes) {
 __device__ inline void lds_dma_b128(u32x4 rsrc, uint32_t lds_addr, uint32_t voffset) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
                :
-               : "s"(lds_addr), "v"(voffset), "s"(rsrc)
+               : "s"(__builtin_amdgcn_readfirstlane((int)lds_addr)), "v"(voffset), "s"(rsrc)
+               : "memory");
+}
+// The 4-byte form: lane l's data lands at lds_addr + 4 l.
+__device__ inline void lds_dma_b32(u32x4 rsrc, uint32_t lds_addr, uint32_t voffset) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, 0 offen lds"
+               :
+               : "s"(__builtin_amdgcn_readfirstlane((int)lds_addr)), "v"(voffset), "s"(rsrc)
                : "memory");
 }
 template <int N>
@@ -252,8 +320,9 @@ struct Tile {
 
 // Moves tiles of ROWS rows from global memory to LDS with NT threads.  Row r of a tile is at base + offset(r), where
 // offset(r) = (r / g) * stride + (r % g) * inner (g rows lie `inner` apart, then `stride`): g = 1 for keys and values, the
-// heads of a group for queries.  DMA: rows of whole 16-byte chunks at 4-byte aligned addresses go straight to LDS;
-// otherwise they pass through registers (fetch before the computation on the tile before, put after it).
+// heads of a group for queries.  DMA: rows at 4-byte aligned addresses go straight to LDS, 16 bytes per lane (the chunk
+// that holds a row's end brings the beginning of the next row along, see `clean`); otherwise they pass through registers
+// (fetch before the computation on the tile before, put after it).
 template <typename T, int DP, int ROWS, int NT, bool DMA>
 struct TileLoader {
   typedef Tile<T, DP> L;
@@ -263,11 +332,16 @@ struct TileLoader {
   u32x4 held[DMA ? 1 : kInstr];
 
   // rows_left: rows of the tile that exist (may be <= 0 or more than ROWS).  first: where the tile's first row lies in
-  // its group of g (0 when g == 1); base is the address of row -first.
+  // its group of g (0 when g == 1); base is the address of row -first (any address when no row exists).
   __device__ inline void fetch(const T *base, int rows_left, uint32_t first, uint32_t g, uint32_t inv_g, uint32_t stride,
                                uint32_t inner, int d, uint32_t lds_addr, int tid) {
     if constexpr (DMA) {
-      const u32x4 rsrc = buffer_words(base, 0x7fffffffu);
+      uint32_t bytes = 0x7fffffffu;
+      if (d % L::kPerChunk != 0) {  // the buffer ends with the last row that exists: nothing behind it is read
+        const uint32_t last = first + (uint32_t)max(0, min(rows_left, ROWS) - 1), t = g == 1 ? last : (last * inv_g) >> 22;
+        bytes = rows_left > 0 ? (t * stride + (last - t * g) * inner + (uint32_t)d) * (uint32_t)sizeof(T) : 0;
+      }
+      const u32x4 rsrc = buffer_words(base, bytes);
       const uint32_t wave_at = (uint32_t)__builtin_amdgcn_readfirstlane((tid & ~63) * 16);
 #pragma unroll
       for (int q = 0; q < kInstr; ++q) {
@@ -282,8 +356,8 @@ struct TileLoader {
         uint32_t off;
         const int slot = q * NT + tid;
         const bool in = place(slot, rows_left, first, g, inv_g, stride, inner, d, &off);
-        const int c = (slot % L::kChunks) ^ L::swizzle(slot / L::kChunks);
-        held[q] = load_chunk(base + (in ? off : 0), in ? d - c * L::kPerChunk : 0);
+        const int c0 = ((slot % L::kChunks) ^ L::swizzle(slot / L::kChunks)) * L::kPerChunk;
+        held[q] = load_part<false, DP == 32>(base + (in ? off - (uint32_t)c0 : 0), in, c0, d);
       }
     }
   }
@@ -291,6 +365,17 @@ struct TileLoader {
     if constexpr (!DMA) {
 #pragma unroll
       for (int q = 0; q < kInstr; ++q) *lds_ptr<u32x4>(lds_addr + (uint32_t)((q * NT + tid) * 16)) = held[q];
+    }
+  }
+  // (DMA, d no whole number of chunks) After a tile has landed: zeros behind every row's end, so that the other operand's
+  // zeros there meet zeros whatever the next row holds.  ROWS threads.
+  __device__ static inline void clean(uint32_t lds_addr, int d, int tid) {
+    if constexpr (DMA) {
+      if (d % L::kPerChunk == 0 || tid >= ROWS) return;
+      const uint32_t chunk = lds_addr + (uint32_t)(tid * L::kPitch) + (uint32_t)(((d / L::kPerChunk) ^ L::swizzle(tid)) << 4);
+#pragma unroll
+      for (int w = 0; w < 4; ++w)  // rows are whole dwords
+        if (w * 4 >= d % L::kPerChunk * (int)sizeof(T)) *lds_ptr<uint32_t>(chunk + 4 * w) = 0;
     }
   }
 
@@ -309,9 +394,30 @@ struct TileLoader {
   }
 };
 
-// ceil(2^22 / g): (r * inverse(g)) >> 22 == r / g for r * g < 2^22.  Rows inside a tile: r < 64 + g, g <= kMostGroup.
+// ceil(2^22 / g): (r * inverse(g)) >> 22 == r / g for r * g < 2^22.  Rows near a tile: r < 192 + g, g <= kMostGroup.
 inline uint32_t inverse(uint32_t g) { return ((1u << 22) + g - 1) / g; }
 constexpr uint32_t kMostGroup = 1024;
+
+// Rows r0, r0 + 1, ... of a key head: row r is query token r / g, head r % g of the group.  `walk` finds the row r0 + i
+// for i < 192 without a division.
+struct RowWalk {
+  uint32_t t0, in0, g, inv_g;
+  // r0 is the same in all lanes, which the compiler cannot always see
+  __device__ inline RowWalk(uint32_t r0, const Shape &s) : g(s.g), inv_g(s.inv_g) {
+    t0 = (uint32_t)__builtin_amdgcn_readfirstlane((int)(r0 / s.g));
+    in0 = (uint32_t)__builtin_amdgcn_readfirstlane((int)(r0 - t0 * s.g));
+  }
+  // where row r0 + i lies among rows of hq heads per token
+  __device__ inline size_t at(uint32_t i, uint32_t hq) const {
+    const uint32_t r = in0 + i, t = (r * inv_g) >> 22;
+    return (size_t)(t0 + t) * hq + (r - t * g);
+  }
+  __device__ inline void advance(uint32_t n) {
+    const uint32_t r = in0 + n, t = (r * inv_g) >> 22;
+    t0 += t;
+    in0 = r - t * g;
+  }
+};
 
 // ---- small things ---------------------------------------------------------------------------------------------------
 
@@ -365,16 +471,22 @@ struct Place {
   SequenceEntry e;
   uint32_t t;
 };
+// The same value in all lanes, which the compiler cannot always see: kept in a scalar register.
+__device__ inline uint32_t uniform(uint32_t x) { return (uint32_t)__builtin_amdgcn_readfirstlane((int)x); }
+__device__ inline SequenceEntry uniform(const SequenceEntry &e) {
+  return {uniform(e.sample), uniform(e.q_start), uniform(e.q_len), uniform(e.k_start), uniform(e.k_len), uniform(e.q_cum),
+          uniform(e.k_cum), 0};
+}
 // rows_per: rows per token (g for queries, 1 for keys); tiles: tiles of a whole sample; by_keys: tiles of keys.
 __device__ inline Place find_place(const SequenceView &s, uint32_t slot, uint32_t tiles, uint32_t size, uint32_t rows_per,
                                    bool by_keys, bool last_first) {
   if (!s.packed) {
     const uint32_t t = slot / s.n;
-    return {s.at(slot - t * s.n), last_first ? tiles - 1 - t : t};
+    return {uniform(s.at(uniform(slot - t * s.n))), uniform(last_first ? tiles - 1 - t : t)};
   }
   const uint32_t total = by_keys ? s.k_total : s.q_total;
   const uint32_t behind = (uint32_t)((uint64_t)total * rows_per / size) + s.n;
-  if (slot >= behind) return {{kNoSequence, 0, 0, 0, 0, 0, 0, 0}, slot - behind};
+  if (slot >= behind) return {{kNoSequence, 0, 0, 0, 0, 0, 0, 0}, uniform(slot - behind)};
   uint32_t lo = 0, hi = s.n;  // the last entry whose first slot is not behind `slot`
   while (hi - lo > 1) {
     const uint32_t mid = (lo + hi) / 2;
@@ -382,10 +494,10 @@ __device__ inline Place find_place(const SequenceView &s, uint32_t slot, uint32_
     if ((uint32_t)((uint64_t)cum * rows_per / size) + mid <= slot) lo = mid;
     else hi = mid;
   }
-  const SequenceEntry e = s.entries[lo];
+  const SequenceEntry e = uniform(s.entries[lo]);
   const uint32_t t = slot - ((uint32_t)((uint64_t)(by_keys ? e.k_cum : e.q_cum) * rows_per / size) + lo);
   const uint32_t own = (uint32_t)(((uint64_t)(by_keys ? e.k_len : e.q_len) * rows_per + size - 1) / size);
-  return {e, last_first && t < own ? own - 1 - t : t};
+  return {e, uniform(last_first && t < own ? own - 1 - t : t)};
 }
 // Slots that find_place can be asked for, per key head.
 inline uint64_t slots(const SequenceView &s, uint32_t size, uint32_t rows_per, bool by_keys) {
@@ -396,13 +508,23 @@ inline uint64_t slots(const SequenceView &s, uint32_t size, uint32_t rows_per, b
 
 // ---- arguments ------------------------------------------------------------------------------------------------------
 
-struct Shape {
-  uint32_t d, hq, hk, g;      // head size, query heads, key heads, hq / hk
-  uint32_t inv_g;
-  uint32_t causal;
-  float scale_log2;           // scale * log2(e): scores are exponents of 2
-  float scale;
-};
+
+// Stages of a wavefront's own ring of pairs of 32-row tiles: four wavefronts take 128 KiB of LDS at most.
+template <typename T, int DP>
+constexpr int kStages = 32 * Tile<T, DP>::kPitch <= 8192 ? 2 : 1;
+
+// Which kernel walks over a call's tiles: the one whose workgroup shares every tile between 128 rows (or keys), or the one
+// where each wavefront walks over tiles of its own, 4 or 1 of them with the same 32 rows (keys).
+enum class Way { Shared, Four, One };
+// wide, narrow: workgroups with tiles of 128 and of 32; most: rows (keys) of the longest sequence; walked: what its
+// workgroups walk over.
+template <typename T>
+inline Way choose_way(phip_ctx *ctx, uint64_t wide, uint64_t narrow, uint64_t most, uint64_t walked) {
+  const uint64_t cus = (uint64_t)ctx->prop.multiProcessorCount;
+  if (sizeof(T) == 4 && most <= 64 && narrow >= 2 * cus) return Way::One;
+  if (wide * 2 <= cus || (sizeof(T) == 4 && wide <= cus && walked >= 1024)) return Way::Four;
+  return Way::Shared;
+}
 
 constexpr uint32_t kMostSize = 128;  // largest head size
 
@@ -413,11 +535,12 @@ inline int make_shape(uint32_t d, uint32_t hq, uint32_t hk, uint32_t tq, uint32_
   PHIP_REQUIRE(hq >= 1 && hk >= 1 && hq % hk == 0, "%u query heads cannot share %u key heads", hq, hk);
   PHIP_REQUIRE(hq / hk <= kMostGroup, "more than %u query heads per key head", kMostGroup);
   PHIP_REQUIRE(tq >= 1 && tk >= 1 && bs >= 1, "empty tensors");
-  PHIP_REQUIRE(tq <= 0x7fffffffu && tk <= 0x7fffffffu, "more than 2^31 - 1 tokens");
+  // rows of a key head (queries times heads of the group) are counted in 32 bits, with room for a tile
+  PHIP_REQUIRE((uint64_t)tq * (hq / hk) <= 0x7fffff00u && tk <= 0x7fffff00u, "more than 2^31 - 256 rows per key head");
   // offsets inside a tile of 64 rows are 32 bits wide
   PHIP_REQUIRE((uint64_t)d * hq * item * 72 < 0x7fffffffu, "heads of %u x %u elements are too large", hq, d);
   PHIP_REQUIRE(scale > 0.f && scale <= 1e30f, "the scale must be positive and at most 1e30");
-  *out = {d, hq, hk, hq / hk, inverse(hq / hk), causal != 0 ? 1u : 0u, scale * kLog2e, scale};
+  *out = {d, hq, hk, hq / hk, inverse(hq / hk), causal != 0 ? 1u : 0u, scale * kLog2e, scale, 0};
   return PHIP_OK;
 }
 
@@ -431,11 +554,12 @@ int allow_lds(phip_ctx *ctx, int bytes) {
   return PHIP_OK;
 }
 
-// True when rows of d elements at all the pointers can be moved in 16-byte chunks that do not reach into the next row.
-inline bool rows_movable(uint32_t d, size_t item, std::initializer_list<const void *> ptrs) {
-  if (d * item % 16 != 0) return false;
+// True when rows of d elements at all the pointers are multiples of `unit` bytes: 4 to be moved to LDS without passing
+// through registers, 16 for plain 16-byte loads.
+inline bool rows_aligned(uint32_t d, size_t item, size_t unit, std::initializer_list<const void *> ptrs) {
+  if (d * item % unit != 0) return false;
   for (const void *p : ptrs)
-    if (reinterpret_cast<uintptr_t>(p) % 16 != 0) return false;
+    if (reinterpret_cast<uintptr_t>(p) % unit != 0) return false;
   return true;
 }
 

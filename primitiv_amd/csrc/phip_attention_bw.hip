@@ -22,7 +22,7 @@ template <typename T>
 struct BwArgs {
   const T *q, *k, *v, *y, *gy;
   const float *stats;
-  float *delta;                 // scratch: one value per row, written by the first kernel
+  float2 *values;               // scratch: per row stats as a power of two, and delta; written by the first kernel
   T *gq, *gk, *gv;
   Shape s;
   SequenceView seq;
@@ -74,39 +74,35 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void queries_kern
   const uint32_t token0 = behind ? a.seq.q_total : e.q_start;
   const size_t sample = behind ? 0 : e.sample;
   const uint32_t tokens = behind ? a.seq.tq - a.seq.q_total : a.seq.packed ? e.q_len : a.seq.tq;
-  const int64_t r0 = (int64_t)at.t * BM;
-  if (r0 >= (int64_t)tokens * sh.g) return;
-  const int lq = behind ? 0 : (int)e.q_len, lk = (int)e.k_len;
+  if ((uint64_t)at.t * BM >= (uint64_t)tokens * sh.g) return;
+  const int lq = behind ? 0 : (int)e.q_len, lk = (int)e.k_len, g = (int)sh.g;
+  const int r0 = (int)at.t * BM, rows = lq * g;
 
-  const int64_t r = r0 + 32 * wave + (lane & 31);
-  const uint32_t tok = (uint32_t)(r / sh.g);
+  const uint32_t r = (uint32_t)(r0 + 32 * wave + (lane & 31)), tok = r / sh.g;
   const bool exists = tok < tokens, valid = exists && (int)tok < lq;
-  const size_t row = ((sample * a.seq.tq + token0 + (exists ? tok : 0)) * sh.hq + head * sh.g + (uint32_t)(r % sh.g));
+  const size_t row = ((sample * a.seq.tq + token0 + (exists ? tok : 0)) * sh.hq + head * sh.g + (r - tok * sh.g));
   const int lim = !valid ? 0 : sh.causal ? min(lk, max(0, (int)tok + lk - lq + 1)) : lk;
 
-  const int64_t last = min((int64_t)lq * sh.g, r0 + BM) - 1;
-  const int wg_keys = last < r0 ? 0 : sh.causal ? min(lk, max(0, (int)(last / sh.g) + lk - lq + 1)) : lk;
-  const int64_t w_first = r0 + 32 * wave, w_last = min((int64_t)lq * sh.g - 1, w_first + 31);
-  int w_keys = 0, w_all = 0;
-  if (w_last >= w_first) {
-    w_keys = sh.causal ? min(lk, max(0, (int)(w_last / sh.g) + lk - lq + 1)) : lk;
-    w_all = sh.causal ? min(lk, max(0, (int)(w_first / sh.g) + lk - lq + 1)) : lk;
-  }
+  auto seen_by = [&](int rr) { return sh.causal ? min(lk, max(0, rr / g + lk - lq + 1)) : lk; };
+  const int last = min(rows, r0 + BM) - 1, wg_keys = last < r0 ? 0 : seen_by(last);
+  const int w_first = r0 + 32 * wave, w_last = min(rows - 1, w_first + 31);
+  const int w_keys = w_last < w_first ? 0 : seen_by(w_last), w_all = w_last < w_first ? 0 : seen_by(w_first);
 
   Frag<T> qf[DP / 16], gf[DP / 16];
   float delta = 0.f;
+  load_row<T>(qf, a.q + row * sh.d, valid, sh, lane);
+  load_row<T>(gf, a.gy + row * sh.d, valid, sh, lane);
+  {
+    Frag<T> yf[DP / 16];
+    load_row<T>(yf, a.y + row * sh.d, valid, sh, lane);
 #pragma unroll
-  for (int c = 0; c < DP / 16; ++c) {
-    const int d0 = 16 * c + 8 * (lane >> 5);
-    qf[c] = load_frag(a.q + row * sh.d, valid, d0, (int)sh.d, (Frag<T> *)nullptr);
-    gf[c] = load_frag(a.gy + row * sh.d, valid, d0, (int)sh.d, (Frag<T> *)nullptr);
-    const Frag<T> yf = load_frag(a.y + row * sh.d, valid, d0, (int)sh.d, (Frag<T> *)nullptr);
+    for (int c = 0; c < DP / 16; ++c)
 #pragma unroll
-    for (int j = 0; j < 8; ++j) delta = fmaf(element(gf[c], j), element(yf, j), delta);
+      for (int j = 0; j < 8; ++j) delta = fmaf(element(gf[c], j), element(yf[c], j), delta);
   }
   delta = halves_sum(delta);
   const float base = valid ? row_base(a.stats[row]) : INFINITY;
-  if (valid && lane < 32) a.delta[row] = delta;
+  if (valid && lane < 32) a.values[row] = {base, delta};
 
   f32x16 acc[DP / 32];
 #pragma unroll
@@ -128,6 +124,11 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void queries_kern
     const uint32_t stage = lds0 + (uint32_t)(t & 1) * 2 * kTile;
     if constexpr (DMA) {
       wait_loads<0>();
+      if (!sh.whole) {  // the parts of the tiles that this thread cleans may be another wavefront's
+        __syncthreads();
+        Loader::clean(stage, (int)sh.d, tid);
+        Loader::clean(stage + kTile, (int)sh.d, tid);
+      }
     } else {
       lk_.put(stage, tid);
       lv_.put(stage + kTile, tid);
@@ -160,6 +161,55 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void queries_kern
   if (exists) emit_row<T, DP>(a.gq + row * sh.d, acc, sh.scale, valid, a.acc_q, sh.d, a.vec != 0, lane);
 }
 
+// What 32 rows (their q at LDS address q_at, gy `to_g` further on, values at `in`) add to the gradients of the wavefront's 32
+// keys.  hidden: rows before it do not see the lane's key.
+template <typename T, int DP>
+__device__ inline void keys_block(f32x16 (&gk)[DP / 32], f32x16 (&gv)[DP / 32], const Frag<T> (&kf)[DP / 16],
+                                  const Frag<T> (&vf)[DP / 16], uint32_t q_at, uint32_t to_g, uint32_t in, bool masked,
+                                  int hidden, float scale_log2, uint32_t row_at, uint32_t col_at, int lane) {
+  typedef Tile<T, DP> L;
+  const uint32_t g_at = q_at + to_g;
+  in += (uint32_t)(4 * (lane >> 5) * 8);
+  hidden -= 4 * (lane >> 5);
+  f32x16 p = f32x16{};
+#pragma unroll
+  for (int c = 0; c < DP / 16; ++c) mma(p, L::row_frag(q_at + row_at, 0, c), kf[c]);
+#pragma unroll
+  for (int i2 = 0; i2 < 8; ++i2) {
+    const f32x4 pair = *lds_ptr<f32x4>(in + (uint32_t)(block_row(2 * i2) * 8));  // two rows: base, delta, base, delta
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const int i = 2 * i2 + e;
+      p[i] = exp2_fast(fmaf(p[i], scale_log2, -pair[2 * e]));
+      if (masked && block_row(i) < hidden) p[i] = 0.f;
+    }
+  }
+#pragma unroll
+  for (int c = 0; c < 2; ++c) {
+    const Frag<T> pf = as_operand(p, c, (Frag<T> *)nullptr);
+#pragma unroll
+    for (int db = 0; db < DP / 32; ++db) mma(gv[db], L::col_frag(g_at + col_at, c, db), pf);
+  }
+  f32x16 dp = f32x16{};
+#pragma unroll
+  for (int c = 0; c < DP / 16; ++c) mma(dp, L::row_frag(g_at + row_at, 0, c), vf[c]);
+#pragma unroll
+  for (int i2 = 0; i2 < 8; ++i2) {
+    const f32x4 pair = *lds_ptr<f32x4>(in + (uint32_t)(block_row(2 * i2) * 8));
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const int i = 2 * i2 + e;
+      dp[i] = p[i] == 0.f ? 0.f : p[i] * (dp[i] - pair[2 * e + 1]);
+    }
+  }
+#pragma unroll
+  for (int c = 0; c < 2; ++c) {
+    const Frag<T> ds = as_operand(dp, c, (Frag<T> *)nullptr);
+#pragma unroll
+    for (int db = 0; db < DP / 32; ++db) mma(gk[db], L::col_frag(q_at + col_at, c, db), ds);
+  }
+}
+
 // gk and gv: a workgroup takes 128 keys, 32 per wavefront, and walks over the rows (queries of the group) that see any of
 // them in tiles of QT.
 template <typename T>
@@ -173,7 +223,7 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 && DMA ? 2 : 1) void keys_
   constexpr uint32_t kTile = (uint32_t)Loader::kBytes;
   extern __shared__ __attribute__((aligned(1024))) unsigned char lds[];
   const uint32_t lds0 = (uint32_t)(size_t)(__attribute__((address_space(3))) unsigned char *)lds;
-  const uint32_t values0 = lds0 + 4 * kTile;  // per stage: QT bases, QT deltas
+  const uint32_t values0 = lds0 + 4 * kTile;  // per stage: QT rows' values
 
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const Shape &sh = a.s;
@@ -184,29 +234,21 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 && DMA ? 2 : 1) void keys_
   const uint32_t token0 = behind ? a.seq.k_total : e.k_start;
   const size_t sample = behind ? 0 : e.sample;
   const uint32_t tokens = behind ? a.seq.tk - a.seq.k_total : a.seq.packed ? e.k_len : a.seq.tk;
-  const int64_t k0 = (int64_t)at.t * BN;
-  if (k0 >= (int64_t)tokens) return;
-  const int lq = (int)e.q_len, lk = behind ? 0 : (int)e.k_len;
-
-  const int64_t key = k0 + 32 * wave + (lane & 31);
-  const bool exists = key < (int64_t)tokens, valid = exists && key < lk;
+  if ((uint64_t)at.t * BN >= (uint64_t)tokens) return;
+  const int lq = (int)e.q_len, lk = behind ? 0 : (int)e.k_len, g = (int)sh.g;
+  const int k0 = (int)at.t * BN, key = k0 + 32 * wave + (lane & 31);
+  const bool exists = key < (int)tokens, valid = exists && key < lk;
   const size_t row = ((sample * a.seq.tk + token0 + (exists ? (uint32_t)key : 0)) * sh.hk + head);
 
   // rows that see any key of the workgroup / the lane's key / any key and all keys of the wavefront: from `*_first` on
-  const int64_t rows = k0 < lk ? (int64_t)lq * sh.g : 0;
-  auto first_row = [&](int64_t kk) { return sh.causal ? max((int64_t)0, kk - (lk - lq)) * (int64_t)sh.g : (int64_t)0; };
-  const int64_t wg_first = first_row(k0) / QT * QT;
-  const int64_t w_k0 = k0 + 32 * wave;
-  const int64_t w_first = w_k0 < lk ? first_row(w_k0) : rows, w_all = first_row(w_k0 + 31);
-  const int64_t my_first = first_row(key);
+  const int rows = k0 < lk ? lq * g : 0;
+  auto first_row = [&](int kk) { return sh.causal ? min(max(0, kk - (lk - lq)), lq) * g : 0; };
+  const int wg_first = first_row(k0) / QT * QT, w_k0 = k0 + 32 * wave;
+  const int w_first = w_k0 < lk ? first_row(w_k0) : rows, w_all = first_row(w_k0 + 31), my_first = first_row(key);
 
   Frag<T> kf[DP / 16], vf[DP / 16];
-#pragma unroll
-  for (int c = 0; c < DP / 16; ++c) {
-    const int d0 = 16 * c + 8 * (lane >> 5);
-    kf[c] = load_frag(a.k + row * sh.d, valid, d0, (int)sh.d, (Frag<T> *)nullptr);
-    vf[c] = load_frag(a.v + row * sh.d, valid, d0, (int)sh.d, (Frag<T> *)nullptr);
-  }
+  load_row<T>(kf, a.k + row * sh.d, valid, sh, lane);
+  load_row<T>(vf, a.v + row * sh.d, valid, sh, lane);
   f32x16 gk[DP / 32], gv[DP / 32];
 #pragma unroll
   for (int db = 0; db < DP / 32; ++db) gk[db] = gv[db] = f32x16{};
@@ -215,31 +257,42 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 && DMA ? 2 : 1) void keys_
   const T *qp = a.q + q_row0 * sh.d, *gp = a.gy + q_row0 * sh.d;
   const uint32_t row_at = L::row_lane(lane), col_at = L::col_lane(lane);
   Loader lq_, lg_;
+  RowWalk walk((uint32_t)wg_first, sh);
   float value = 0.f;
-  auto fetch = [&](int64_t r, int stage_no) {
+  // the tile of rows from r on, where the walk stands, into a stage; the values of a row side by side
+  auto fetch = [&](int r, int stage_no) {
     const uint32_t stage = lds0 + (uint32_t)stage_no * 2 * kTile;
-    const uint32_t t0 = (uint32_t)(r / sh.g), in_group = (uint32_t)(r % sh.g);
-    const size_t off = (size_t)t0 * sh.hq * sh.d;
-    const int left = (int)min((int64_t)QT, rows - r);
-    lq_.fetch(qp + off, left, in_group, sh.g, sh.inv_g, sh.hq * sh.d, sh.d, (int)sh.d, stage, tid);
-    lg_.fetch(gp + off, left, in_group, sh.g, sh.inv_g, sh.hq * sh.d, sh.d, (int)sh.d, stage + kTile, tid);
-    if (tid < 2 * QT) {
-      const int i = tid & (QT - 1);
-      const uint32_t rr = in_group + (uint32_t)i, t = (rr * sh.inv_g) >> 22;
-      const size_t w = q_row0 + (size_t)(t0 + t) * sh.hq + (rr - t * sh.g);
-      value = tid < QT ? INFINITY : 0.f;
-      if (i < left) value = tid < QT ? row_base(a.stats[w]) : a.delta[w];
+    const size_t off = (size_t)walk.t0 * sh.hq * sh.d;
+    const int left = min(QT, rows - r);
+    lq_.fetch(qp + off, left, walk.in0, sh.g, sh.inv_g, sh.hq * sh.d, sh.d, (int)sh.d, stage, tid);
+    lg_.fetch(gp + off, left, walk.in0, sh.g, sh.inv_g, sh.hq * sh.d, sh.d, (int)sh.d, stage + kTile, tid);
+    // rows past the end get zeros, which with their zeros for q and gy add nothing
+    const bool in = (tid >> 1) < left;
+    const float *p = reinterpret_cast<const float *>(a.values + q_row0 + (size_t)walk.t0 * sh.hq);
+    const uint32_t rr = walk.in0 + ((uint32_t)tid >> 1), t = (rr * sh.inv_g) >> 22;
+    const uint32_t at_value = 2 * (t * sh.hq + (rr - t * sh.g)) + (tid & 1);
+    if (wave < 2 * QT / 64) {
+      if constexpr (DMA)
+        lds_dma_b32(buffer_words(p, 0x7fffffffu), values0 + (uint32_t)((stage_no * 2 * QT + wave * 64) * 4), in ? at_value * 4 : kOutOfRange);
+      else
+        value = in ? p[at_value] : 0.f;
     }
+    walk.advance(QT);
   };
   if (wg_first < rows) fetch(wg_first, 0);
   int s = 0;
-  for (int64_t r = wg_first; r < rows; r += QT, s ^= 1) {
+  for (int r = wg_first; r < rows; r += QT, s ^= 1) {
     const uint32_t stage = lds0 + (uint32_t)s * 2 * kTile;
     const uint32_t values = values0 + (uint32_t)(s * 2 * QT * 4);
-    if (tid < 2 * QT) *lds_ptr<float>(values + (uint32_t)tid * 4) = value;
     if constexpr (DMA) {
       wait_loads<0>();
+      if (!sh.whole) {  // the parts of the tiles that this thread cleans may be another wavefront's
+        __syncthreads();
+        Loader::clean(stage, (int)sh.d, tid);
+        Loader::clean(stage + kTile, (int)sh.d, tid);
+      }
     } else {
+      if (tid < 2 * QT) *lds_ptr<float>(values + (uint32_t)tid * 4) = value;
       lq_.put(stage, tid);
       lg_.put(stage + kTile, tid);
     }
@@ -249,46 +302,8 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 && DMA ? 2 : 1) void keys_
     const bool masked = r < w_all;
 #pragma unroll 1
     for (int qb = 0; qb < QT / 32; ++qb) {
-      const uint32_t q_at = stage + (uint32_t)(qb * 32 * L::kPitch), g_at = q_at + kTile;
-      const uint32_t in = values + (uint32_t)((32 * qb + 4 * (lane >> 5)) * 4);
-      const int hidden = (int)max((int64_t)0, min((int64_t)QT, my_first - r)) - 32 * qb - 4 * (lane >> 5);
-      f32x16 p = f32x16{};
-#pragma unroll
-      for (int c = 0; c < DP / 16; ++c) mma(p, L::row_frag(q_at + row_at, 0, c), kf[c]);
-#pragma unroll
-      for (int i4 = 0; i4 < 4; ++i4) {
-        const f32x4 base = *lds_ptr<f32x4>(in + 32 * i4);
-#pragma unroll
-        for (int e4 = 0; e4 < 4; ++e4) {
-          const int i = 4 * i4 + e4;
-          p[i] = exp2_fast(fmaf(p[i], sh.scale_log2, -base[e4]));
-          if (masked && block_row(i) < hidden) p[i] = 0.f;
-        }
-      }
-#pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        const Frag<T> pf = as_operand(p, c, (Frag<T> *)nullptr);
-#pragma unroll
-        for (int db = 0; db < DP / 32; ++db) mma(gv[db], L::col_frag(g_at + col_at, c, db), pf);
-      }
-      f32x16 dp = f32x16{};
-#pragma unroll
-      for (int c = 0; c < DP / 16; ++c) mma(dp, L::row_frag(g_at + row_at, 0, c), vf[c]);
-#pragma unroll
-      for (int i4 = 0; i4 < 4; ++i4) {
-        const f32x4 delta = *lds_ptr<f32x4>(in + QT * 4 + 32 * i4);
-#pragma unroll
-        for (int e4 = 0; e4 < 4; ++e4) {
-          const int i = 4 * i4 + e4;
-          dp[i] = p[i] == 0.f ? 0.f : p[i] * (dp[i] - delta[e4]);
-        }
-      }
-#pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        const Frag<T> ds = as_operand(dp, c, (Frag<T> *)nullptr);
-#pragma unroll
-        for (int db = 0; db < DP / 32; ++db) mma(gk[db], L::col_frag(q_at + col_at, c, db), ds);
-      }
+      keys_block<T, DP>(gk, gv, kf, vf, stage + (uint32_t)(qb * 32 * L::kPitch), kTile, values + (uint32_t)(qb * 32 * 8), masked,
+                        min(QT, my_first - r) - 32 * qb, sh.scale_log2, row_at, col_at, lane);
     }
   }
   if (!exists) return;
@@ -297,32 +312,292 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 && DMA ? 2 : 1) void keys_
   emit_row<T, DP>(a.gv + row * sh.d, gv, 1.f, valid, a.acc_v, sh.d, a.vec != 0, lane);
 }
 
-template <typename T, int DP, bool DMA>
-int launch(phip_ctx *ctx, BwArgs<T> a) {
-  constexpr int BM = 32 * kWaves;
-  constexpr int lds_q = 4 * kKeys<T> * Tile<T, DP>::kPitch;
-  constexpr int lds_k = 4 * kRows<T> * Tile<T, DP>::kPitch + 4 * kRows<T> * 4;
-  int rc = allow_lds<queries_kernel<T, DP, DMA>>(ctx, lds_q);
-  if (rc == PHIP_OK) rc = allow_lds<keys_kernel<T, DP, DMA>>(ctx, lds_k);
+// The same two for few tiles (short sequences, few heads): a workgroup of W wavefronts takes 32 queries (32 keys) and its
+// wavefronts walk over blocks of 32 keys (rows) of their own, through rings of LDS tiles of their own; their sums meet in
+// LDS at the end, in a fixed order.  With W = 1 a workgroup is one wavefront, for sequences so short that there is nothing
+// to divide.
+template <typename T, int DP, int W>
+constexpr int kFewLds = W * std::max(2 * kStages<T, DP> * 32 * Tile<T, DP>::kPitch + 2 * kStages<T, DP> * 32 * 4, DP * 33 * 4);
+
+// Adds the wavefronts' blocks (rows of the result across) through LDS and writes the 32 rows, four elements per thread at
+// a time.  row(r): where row r goes, null where it does not exist; of these the first `filled` have a gradient.
+template <typename T, int DP, int W, typename Row>
+__device__ inline void emit_sum(const f32x16 (&x)[DP / 32], unsigned char *lds, float f, uint32_t acc, uint32_t d, bool vec,
+                                Row row, int filled) {
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  if constexpr (W == 1) {
+    T *p = row(lane & 31);
+    if (p != nullptr) emit_row<T, DP>(p, x, f, (lane & 31) < filled, acc, d, vec, lane);
+    return;
+  }
+  constexpr int kPer = DP * 33;
+  float *const area = reinterpret_cast<float *>(lds);
+  __syncthreads();
+#pragma unroll
+  for (int db = 0; db < DP / 32; ++db)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) area[wave * kPer + (32 * db + block_row(i) + 4 * (lane >> 5)) * 33 + (lane & 31)] = x[db][i];
+  __syncthreads();
+#pragma unroll
+  for (uint32_t i = tid; i < 32 * (DP / 4); i += 64 * W) {
+    const int r = (int)(i / (DP / 4));
+    const uint32_t dd = i % (DP / 4) * 4;
+    T *p = row(r);
+    const bool valid = r < filled;
+    if (p == nullptr || dd >= d || (acc && !valid)) continue;
+    float four[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      float sum = 0.f;
+#pragma unroll
+      for (int w = 0; w < W; ++w) sum += area[w * kPer + (dd + e) * 33 + r];
+      four[e] = valid ? sum * f : 0.f;
+    }
+    if (acc) store4<T, true>(p + dd, four, (int)(d - dd), vec);
+    else store4<T, false>(p + dd, four, (int)(d - dd), vec);
+  }
+}
+
+template <typename T, int DP, bool DMA, int W>
+__global__ __launch_bounds__(64 * W, 1) void few_queries_kernel(const BwArgs<T> a) {
+  constexpr int BM = 32, S = DMA ? kStages<T, DP> : 1;
+  typedef Tile<T, DP> L;
+  typedef TileLoader<T, DP, 32, 64, DMA> Loader;
+  constexpr uint32_t kTile = (uint32_t)Loader::kBytes;
+  extern __shared__ __attribute__((aligned(1024))) unsigned char lds[];
+  const uint32_t lds0 = (uint32_t)(size_t)(__attribute__((address_space(3))) unsigned char *)lds;
+
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const Shape &sh = a.s;
+  const uint32_t head = blockIdx.x % sh.hk, slot = blockIdx.x / sh.hk;
+  const Place at = find_place(a.seq, slot, a.tiles, BM, sh.g, false, sh.causal != 0);
+  const SequenceEntry &e = at.e;
+  const bool behind = e.sample == kNoSequence;
+  const uint32_t token0 = behind ? a.seq.q_total : e.q_start;
+  const size_t sample = behind ? 0 : e.sample;
+  const uint32_t tokens = behind ? a.seq.tq - a.seq.q_total : a.seq.packed ? e.q_len : a.seq.tq;
+  if ((uint64_t)at.t * BM >= (uint64_t)tokens * sh.g) return;
+  const int lq = behind ? 0 : (int)e.q_len, lk = (int)e.k_len, g = (int)sh.g;
+  const int r0 = (int)at.t * BM, rows = lq * g;
+  // the lane's row; keys that it, any row and all rows of the tile see
+  const int exist = min((int)(tokens * sh.g) - r0, BM), filled = min(rows - r0, BM);
+  auto seen_by = [&](int rr) { return sh.causal ? min(lk, max(0, rr / g + lk - lq + 1)) : lk; };
+  const bool valid = (lane & 31) < filled;
+  const int lim = valid ? seen_by(r0 + (lane & 31)) : 0;
+  const int keys = filled <= 0 ? 0 : seen_by(r0 + filled - 1), all = filled <= 0 ? 0 : seen_by(r0);
+  const RowWalk walk((uint32_t)r0, sh);
+  const size_t row_0 = (sample * a.seq.tq + token0) * sh.hq + head * sh.g;
+  const size_t row = row_0 + walk.at(valid ? lane & 31 : 0, sh.hq);
+
+  const uint32_t stride = sh.hk * sh.d;
+  const T *kp = a.k + ((sample * a.seq.tk + e.k_start) * sh.hk + head) * (size_t)sh.d;
+  const T *vp = a.v + ((sample * a.seq.tk + e.k_start) * sh.hk + head) * (size_t)sh.d;
+  const uint32_t ring = lds0 + (uint32_t)wave * (2 * S * kTile);
+  const uint32_t row_at = L::row_lane(lane), col_at = L::col_lane(lane);
+  constexpr int kStep = 32 * W;
+  Loader lk_, lv_;
+  auto fetch = [&](int key, int s) {
+    const size_t off = (size_t)min(key, keys) * stride;
+    lk_.fetch(kp + off, keys - key, 0, 1, 0, stride, 0, (int)sh.d, ring + (uint32_t)s * 2 * kTile, lane);
+    lv_.fetch(vp + off, keys - key, 0, 1, 0, stride, 0, (int)sh.d, ring + (uint32_t)s * 2 * kTile + kTile, lane);
+  };
+  Frag<T> qf[DP / 16], gf[DP / 16];
+  float delta = 0.f;
+  load_row<T>(qf, a.q + row * sh.d, valid, sh, lane);
+  load_row<T>(gf, a.gy + row * sh.d, valid, sh, lane);
+  {
+    Frag<T> yf[DP / 16];
+    load_row<T>(yf, a.y + row * sh.d, valid, sh, lane);
+#pragma unroll
+    for (int c = 0; c < DP / 16; ++c)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) delta = fmaf(element(gf[c], j), element(yf[c], j), delta);
+  }
+  int key = 32 * wave;
+#pragma unroll
+  for (int s = 0; s < S; ++s) fetch(key + s * kStep, s);
+
+  delta = halves_sum(delta);
+  const float base = valid ? row_base(a.stats[row]) : INFINITY;
+  if (valid && tid < 32) a.values[row] = {base, delta};
+
+  arrived(qf);
+  arrived(gf);
+  f32x16 acc[DP / 32];
+#pragma unroll
+  for (int db = 0; db < DP / 32; ++db) acc[db] = f32x16{};
+  for (int s = 0; key < keys; key += kStep, s = s + 1 == S ? 0 : s + 1) {
+    const uint32_t stage = ring + (uint32_t)s * 2 * kTile;
+    if constexpr (DMA) {
+      wait_loads<(S - 1) * 2 * Loader::kInstr>();
+      if (!sh.whole) {
+        Loader::clean(stage, (int)sh.d, lane);
+        Loader::clean(stage + kTile, (int)sh.d, lane);
+      }
+    } else {
+      lk_.put(stage, lane);
+      lv_.put(stage + kTile, lane);
+      fetch(key + kStep, 0);
+    }
+    f32x16 p = f32x16{}, dp = f32x16{};
+#pragma unroll
+    for (int c = 0; c < DP / 16; ++c) mma(p, L::row_frag(stage + row_at, 0, c), qf[c]);
+#pragma unroll
+    for (int c = 0; c < DP / 16; ++c) mma(dp, L::row_frag(stage + kTile + row_at, 0, c), gf[c]);
+    const bool masked = key + 32 > all;
+    const int first = key + 4 * (lane >> 5);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const float x = exp2_fast(fmaf(p[i], sh.scale_log2, -base)) * (dp[i] - delta);
+      p[i] = masked && first + block_row(i) >= lim ? 0.f : x;
+    }
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      const Frag<T> ds = as_operand(p, c, (Frag<T> *)nullptr);
+#pragma unroll
+      for (int db = 0; db < DP / 32; ++db) mma(acc[db], L::col_frag(stage + col_at, c, db), ds);
+    }
+    if constexpr (DMA) {
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the tile's reads are done before its place is filled again
+      fetch(key + S * kStep, s);
+    }
+  }
+  wait_loads<0>();
+  emit_sum<T, DP, W>(acc, lds, sh.scale, a.acc_q, sh.d, a.vec != 0,
+                     [&](int i) { return i < exist ? a.gq + (row_0 + walk.at((uint32_t)i, sh.hq)) * sh.d : (T *)nullptr; },
+                     filled);
+}
+
+template <typename T, int DP, bool DMA, int W>
+__global__ __launch_bounds__(64 * W, 1) void few_keys_kernel(const BwArgs<T> a) {
+  constexpr int BN = 32, S = DMA ? kStages<T, DP> : 1;
+  typedef Tile<T, DP> L;
+  typedef TileLoader<T, DP, 32, 64, DMA> Loader;
+  constexpr uint32_t kTile = (uint32_t)Loader::kBytes;
+  extern __shared__ __attribute__((aligned(1024))) unsigned char lds[];
+  const uint32_t lds0 = (uint32_t)(size_t)(__attribute__((address_space(3))) unsigned char *)lds;
+
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const Shape &sh = a.s;
+  const uint32_t head = blockIdx.x % sh.hk, slot = blockIdx.x / sh.hk;
+  const Place at = find_place(a.seq, slot, a.tiles, BN, 1, true, false);
+  const SequenceEntry &e = at.e;
+  const bool behind = e.sample == kNoSequence;
+  const uint32_t token0 = behind ? a.seq.k_total : e.k_start;
+  const size_t sample = behind ? 0 : e.sample;
+  const uint32_t tokens = behind ? a.seq.tk - a.seq.k_total : a.seq.packed ? e.k_len : a.seq.tk;
+  if ((uint64_t)at.t * BN >= (uint64_t)tokens) return;
+  const int lq = (int)e.q_len, lk = behind ? 0 : (int)e.k_len, g = (int)sh.g;
+  const int k0 = (int)at.t * BN, key = k0 + (lane & 31), exist = min((int)tokens - k0, BN);
+  const bool valid = key < lk;
+  const size_t row_0 = (sample * a.seq.tk + token0 + (uint32_t)k0) * sh.hk + head;  // keys lie hk rows apart
+  const size_t row = row_0 + (valid ? (size_t)(lane & 31) * sh.hk : 0);
+  const int rows = k0 < lk ? lq * g : 0;
+  auto first_row = [&](int kk) { return sh.causal ? min(max(0, kk - (lk - lq)), lq) * g : 0; };
+  const int all = first_row(k0 + 31), my_first = first_row(key);
+
+  const size_t q_row0 = (sample * a.seq.tq + e.q_start) * sh.hq + head * sh.g;
+  const T *qp = a.q + q_row0 * sh.d, *gp = a.gy + q_row0 * sh.d;
+  const uint32_t ring = lds0 + (uint32_t)wave * (2 * S * kTile);
+  const uint32_t values0 = lds0 + (uint32_t)W * (2 * S * kTile) + (uint32_t)wave * (S * 64 * 4);
+  const uint32_t row_at = L::row_lane(lane), col_at = L::col_lane(lane);
+  constexpr int kStep = 32 * W;
+  Loader lq_, lg_;
+  float value = 0.f;
+  int rr = first_row(k0) / 32 * 32 + 32 * wave;
+  RowWalk walk((uint32_t)rr, sh);
+  // the rows from `from` on, where the walk stands, into stage s; lane 2 i + e brings value e of row i
+  auto fetch = [&](int from, int s) {
+    const size_t off = from < rows ? (size_t)walk.t0 * sh.hq * sh.d : 0;
+    const int left = min(32, rows - from);
+    const uint32_t stage = ring + (uint32_t)s * 2 * kTile;
+    lq_.fetch(qp + off, left, walk.in0, sh.g, sh.inv_g, sh.hq * sh.d, sh.d, (int)sh.d, stage, lane);
+    lg_.fetch(gp + off, left, walk.in0, sh.g, sh.inv_g, sh.hq * sh.d, sh.d, (int)sh.d, stage + kTile, lane);
+    const bool in = (lane >> 1) < left;
+    const float *p = reinterpret_cast<const float *>(a.values + q_row0 + (from < rows ? (size_t)walk.t0 * sh.hq : 0));
+    const uint32_t r = walk.in0 + ((uint32_t)lane >> 1), t = (r * sh.inv_g) >> 22;
+    const uint32_t at_value = 2 * (t * sh.hq + (r - t * sh.g)) + (lane & 1);
+    if constexpr (DMA) lds_dma_b32(buffer_words(p, 0x7fffffffu), values0 + (uint32_t)(s * 64 * 4), in ? at_value * 4 : kOutOfRange);
+    else value = in ? p[at_value] : 0.f;
+    walk.advance(kStep);
+  };
+  Frag<T> kf[DP / 16], vf[DP / 16];
+  load_row<T>(kf, a.k + row * sh.d, valid, sh, lane);
+  load_row<T>(vf, a.v + row * sh.d, valid, sh, lane);
+#pragma unroll
+  for (int s = 0; s < S; ++s) fetch(rr + s * kStep, s);
+
+  arrived(kf);
+  arrived(vf);
+  f32x16 gk[DP / 32], gv[DP / 32];
+#pragma unroll
+  for (int db = 0; db < DP / 32; ++db) gk[db] = gv[db] = f32x16{};
+
+  for (int s = 0; rr < rows; rr += kStep, s = s + 1 == S ? 0 : s + 1) {
+    const uint32_t stage = ring + (uint32_t)s * 2 * kTile, in = values0 + (uint32_t)(s * 64 * 4);
+    if constexpr (DMA) {
+      wait_loads<(S - 1) * (2 * Loader::kInstr + 1)>();
+      if (!sh.whole) {
+        Loader::clean(stage, (int)sh.d, lane);
+        Loader::clean(stage + kTile, (int)sh.d, lane);
+      }
+    } else {
+      lq_.put(stage, lane);
+      lg_.put(stage + kTile, lane);
+      *lds_ptr<float>(in + (uint32_t)lane * 4) = value;
+      fetch(rr + kStep, 0);
+    }
+    keys_block<T, DP>(gk, gv, kf, vf, stage, kTile, in, rr < all, my_first - rr, sh.scale_log2, row_at, col_at, lane);
+    if constexpr (DMA) {
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the tile's reads are done before its place is filled again
+      fetch(rr + S * kStep, s);
+    }
+  }
+  wait_loads<0>();
+  auto in_k = [&](int i) { return i < exist ? a.gk + (row_0 + (size_t)i * sh.hk) * sh.d : (T *)nullptr; };
+  auto in_v = [&](int i) { return i < exist ? a.gv + (row_0 + (size_t)i * sh.hk) * sh.d : (T *)nullptr; };
+  // the two gradients may be one tensor: one after the other, by the same thread
+  emit_sum<T, DP, W>(gk, lds, sh.scale, a.acc_k, sh.d, a.vec != 0, in_k, lk - k0);
+  emit_sum<T, DP, W>(gv, lds, 1.f, a.acc_v, sh.d, a.vec != 0, in_v, lk - k0);
+}
+
+template <auto *KERNEL, typename T>
+int launch_kernel(phip_ctx *ctx, const BwArgs<T> &a, uint64_t blocks, int threads, int lds) {
+  const int rc = allow_lds<KERNEL>(ctx, lds);
   if (rc != PHIP_OK) return rc;
-  const uint64_t blocks_q = slots(a.seq, BM, a.s.g, false) * a.s.hk, blocks_k = slots(a.seq, BM, 1, true) * a.s.hk;
-  PHIP_REQUIRE(blocks_q < 0x7fffffffu && blocks_k < 0x7fffffffu, "too many rows");
-  a.tiles = (uint32_t)(((uint64_t)a.seq.tq * a.s.g + BM - 1) / BM);
-  hipLaunchKernelGGL((queries_kernel<T, DP, DMA>), dim3((uint32_t)blocks_q), dim3(kThreads), lds_q, ctx->stream, a);
-  PHIP_LAUNCH_CHECK();
-  a.tiles = (uint32_t)((a.seq.tk + BM - 1) / BM);
-  hipLaunchKernelGGL((keys_kernel<T, DP, DMA>), dim3((uint32_t)blocks_k), dim3(kThreads), lds_k, ctx->stream, a);
+  PHIP_REQUIRE(blocks < 0x7fffffffu, "too many rows");
+  hipLaunchKernelGGL(KERNEL, dim3((uint32_t)blocks), dim3((uint32_t)threads), lds, ctx->stream, a);
   PHIP_LAUNCH_CHECK();
   return PHIP_OK;
 }
 
+template <typename T, int DP, bool DMA>
+int launch(phip_ctx *ctx, BwArgs<T> a, const phip_sequences *seqs) {
+  constexpr int lds_q = 4 * kKeys<T> * Tile<T, DP>::kPitch;
+  constexpr int lds_k = 4 * kRows<T> * Tile<T, DP>::kPitch + 4 * kRows<T> * 4;
+  const uint64_t most_q = (uint64_t)(seqs != nullptr ? seqs->max_q : a.seq.tq) * a.s.g, most_k = seqs != nullptr ? seqs->max_k : a.seq.tk;
+  const uint64_t wide_q = slots(a.seq, 128, a.s.g, false) * a.s.hk, narrow_q = slots(a.seq, 32, a.s.g, false) * a.s.hk;
+  const uint64_t wide_k = slots(a.seq, 128, 1, true) * a.s.hk, narrow_k = slots(a.seq, 32, 1, true) * a.s.hk;
+  const Way way_q = choose_way<T>(ctx, wide_q, narrow_q, most_q, most_k), way_k = choose_way<T>(ctx, wide_k, narrow_k, most_k, most_q);
+  const uint64_t rows = (uint64_t)a.seq.tq * a.s.g, keys = a.seq.tk;
+  a.tiles = (uint32_t)(way_q == Way::Shared ? (rows + 127) / 128 : (rows + 31) / 32);
+  int rc = way_q == Way::Shared ? launch_kernel<queries_kernel<T, DP, DMA>>(ctx, a, wide_q, kThreads, lds_q)
+           : way_q == Way::Four ? launch_kernel<few_queries_kernel<T, DP, DMA, 4>>(ctx, a, narrow_q, 256, kFewLds<T, DP, 4>)
+                                : launch_kernel<few_queries_kernel<T, DP, DMA, 1>>(ctx, a, narrow_q, 64, kFewLds<T, DP, 1>);
+  if (rc != PHIP_OK) return rc;
+  a.tiles = (uint32_t)(way_k == Way::Shared ? (keys + 127) / 128 : (keys + 31) / 32);
+  return way_k == Way::Shared ? launch_kernel<keys_kernel<T, DP, DMA>>(ctx, a, wide_k, kThreads, lds_k)
+         : way_k == Way::Four ? launch_kernel<few_keys_kernel<T, DP, DMA, 4>>(ctx, a, narrow_k, 256, kFewLds<T, DP, 4>)
+                              : launch_kernel<few_keys_kernel<T, DP, DMA, 1>>(ctx, a, narrow_k, 64, kFewLds<T, DP, 1>);
+}
+
 template <typename T>
-int dispatch(phip_ctx *ctx, const BwArgs<T> &a, bool dma) {
+int dispatch(phip_ctx *ctx, const BwArgs<T> &a, const phip_sequences *seqs, bool dma) {
   switch ((a.s.d + 31) / 32) {
-    case 1: return dma ? launch<T, 32, true>(ctx, a) : launch<T, 32, false>(ctx, a);
-    case 2: return dma ? launch<T, 64, true>(ctx, a) : launch<T, 64, false>(ctx, a);
-    case 3: return dma ? launch<T, 96, true>(ctx, a) : launch<T, 96, false>(ctx, a);
-    default: return dma ? launch<T, 128, true>(ctx, a) : launch<T, 128, false>(ctx, a);
+    case 1: return dma ? launch<T, 32, true>(ctx, a, seqs) : launch<T, 32, false>(ctx, a, seqs);
+    case 2: return dma ? launch<T, 64, true>(ctx, a, seqs) : launch<T, 64, false>(ctx, a, seqs);
+    case 3: return dma ? launch<T, 96, true>(ctx, a, seqs) : launch<T, 96, false>(ctx, a, seqs);
+    default: return dma ? launch<T, 128, true>(ctx, a, seqs) : launch<T, 128, false>(ctx, a, seqs);
   }
 }
 
@@ -356,8 +631,8 @@ int backward(phip_ctx *ctx, const T *q, const T *k, const T *v, const T *y, cons
   a.acc_k = !zeros_take(ctx, gk, nk);
   a.acc_v = !zeros_take(ctx, gv, nk);
   PHIP_FLUSH_ZEROS(ctx);
-  void *delta = nullptr;
-  rc = phip_pool_alloc(ctx, ns, &delta, nullptr);
+  void *values = nullptr;
+  rc = phip_pool_alloc(ctx, 2 * ns, &values, nullptr);
   if (rc != PHIP_OK) return rc;
   a.q = q;
   a.k = k;
@@ -365,14 +640,15 @@ int backward(phip_ctx *ctx, const T *q, const T *k, const T *v, const T *y, cons
   a.y = y;
   a.gy = gy;
   a.stats = stats;
-  a.delta = static_cast<float *>(delta);
+  a.values = static_cast<float2 *>(values);
   a.gq = gq;
   a.gk = gk;
   a.gv = gv;
   auto vec = [&](const void *p) { return reinterpret_cast<uintptr_t>(p) % (4 * sizeof(T)) == 0; };
   a.vec = d % 4 == 0 && vec(gq) && vec(gk) && vec(gv);
-  rc = dispatch<T>(ctx, a, rows_movable(d, sizeof(T), {q, k, v, gy}));
-  phip_pool_free(ctx, delta);
+  a.s.whole = rows_aligned(d, sizeof(T), 16, {q, k, v, y, gy});
+  rc = dispatch<T>(ctx, a, seqs, rows_aligned(d, sizeof(T), 4, {q, k, v, y, gy}));
+  phip_pool_free(ctx, values);
   return rc;
 }
 

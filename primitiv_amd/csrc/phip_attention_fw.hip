@@ -149,31 +149,24 @@ __global__ __launch_bounds__(kThreads, 2) void rows_kernel(const FwArgs<T> a) {
   const uint32_t token0 = behind ? a.seq.q_total : e.q_start;  // of the sample
   const size_t sample = behind ? 0 : e.sample;
   const uint32_t tokens = behind ? a.seq.tq - a.seq.q_total : a.seq.packed ? e.q_len : a.seq.tq;  // that this workgroup writes
-  const int64_t r0 = (int64_t)at.t * BM;
-  if (r0 >= (int64_t)tokens * sh.g) return;
-  const int lq = behind ? 0 : (int)e.q_len, lk = (int)e.k_len;
+  if ((uint64_t)at.t * BM >= (uint64_t)tokens * sh.g) return;
+  const int lq = behind ? 0 : (int)e.q_len, lk = (int)e.k_len, g = (int)sh.g;
+  const int r0 = (int)at.t * BM, rows = lq * g;
 
   // the lane's row
-  const int64_t r = r0 + 32 * wave + (lane & 31);
-  const uint32_t tok = (uint32_t)(r / sh.g);
+  const uint32_t r = (uint32_t)(r0 + 32 * wave + (lane & 31)), tok = r / sh.g;
   const bool exists = tok < tokens, valid = exists && (int)tok < lq;
-  const size_t row = ((sample * a.seq.tq + token0 + (exists ? tok : 0)) * sh.hq + head * sh.g + (uint32_t)(r % sh.g));
+  const size_t row = ((sample * a.seq.tq + token0 + (exists ? tok : 0)) * sh.hq + head * sh.g + (r - tok * sh.g));
   const int lim = !valid ? 0 : sh.causal ? min(lk, max(0, (int)tok + lk - lq + 1)) : lk;
 
   // keys that any row of the workgroup, all rows of the wavefront, any row of the wavefront sees
-  const int64_t last = min((int64_t)lq * sh.g, r0 + BM) - 1;
-  const int wg_keys = last < r0 ? 0 : sh.causal ? min(lk, max(0, (int)(last / sh.g) + lk - lq + 1)) : lk;
-  const int64_t w_first = r0 + 32 * wave, w_last = min((int64_t)lq * sh.g - 1, w_first + 31);
-  int w_keys = 0, w_all = 0;
-  if (w_last >= w_first) {
-    w_keys = sh.causal ? min(lk, max(0, (int)(w_last / sh.g) + lk - lq + 1)) : lk;
-    w_all = sh.causal ? min(lk, max(0, (int)(w_first / sh.g) + lk - lq + 1)) : lk;
-  }
+  auto seen_by = [&](int rr) { return sh.causal ? min(lk, max(0, rr / g + lk - lq + 1)) : lk; };
+  const int last = min(rows, r0 + BM) - 1, wg_keys = last < r0 ? 0 : seen_by(last);
+  const int w_first = r0 + 32 * wave, w_last = min(rows - 1, w_first + 31);
+  const int w_keys = w_last < w_first ? 0 : seen_by(w_last), w_all = w_last < w_first ? 0 : seen_by(w_first);
 
   Frag<T> qf[DP / 16];
-#pragma unroll
-  for (int c = 0; c < DP / 16; ++c)
-    qf[c] = load_frag(a.q + row * sh.d, valid, 16 * c + 8 * (lane >> 5), (int)sh.d, (Frag<T> *)nullptr);
+  load_row<T>(qf, a.q + row * sh.d, valid, sh, lane);
 
   Rows<DP> st;
   reset(st);
@@ -194,6 +187,10 @@ __global__ __launch_bounds__(kThreads, 2) void rows_kernel(const FwArgs<T> a) {
     const uint32_t stage = lds0 + (uint32_t)(t & 1) * 2 * kTile;
     if constexpr (DMA) {
       wait_loads<0>();
+      if (!sh.whole) {  // the parts of the tile that this thread cleans may be another wavefront's
+        __syncthreads();
+        Loader::clean(stage, (int)sh.d, tid);
+      }
     } else {
       lk_.put(stage, tid);
       lv_.put(stage + kTile, tid);
@@ -222,10 +219,8 @@ __global__ __launch_bounds__(kThreads, 2) void rows_kernel(const FwArgs<T> a) {
 // Every wavefront has a ring of LDS tiles of its own and waits for nobody else: K and V blocks alternate in it, and the
 // block `kRing` positions ahead is ordered as soon as a block has been used, so that up to three quarters of 128 KiB are on
 // their way to every CU.
-template <typename T, int DP>
-constexpr int kStages = 32 * Tile<T, DP>::kPitch <= 8192 ? 2 : 1;  // pairs of K and V: 128 KiB of LDS at most
-template <typename T, int DP>
-constexpr int kFewLds = std::max(kWaves * 2 * kStages<T, DP> * 32 * Tile<T, DP>::kPitch, kWaves * (DP * 33 + 64) * 4);
+template <typename T, int DP, int W>
+constexpr int kFewLds = W * std::max(2 * kStages<T, DP> * 32 * Tile<T, DP>::kPitch, (DP * 33 + 64) * 4);
 
 // Device-scope accesses for what travels between workgroups, which may sit behind different L2 caches.
 __device__ inline void store_shared(float *p, float x) {
@@ -251,9 +246,9 @@ __device__ inline bool last_of_tile(uint32_t *ticket, uint32_t count, uint32_t *
   return *flag != 0;
 }
 
-template <typename T, int DP, bool DMA>
-__global__ __launch_bounds__(kThreads, 1) void few_kernel(const FwArgs<T> a) {
-  constexpr int BM = 32, S = kStages<T, DP>;
+template <typename T, int DP, bool DMA, int W>
+__global__ __launch_bounds__(64 * W, 1) void few_kernel(const FwArgs<T> a) {
+  constexpr int BM = 32, S = kStages<T, DP>, kThreads = 64 * W;
   typedef Tile<T, DP> L;
   typedef TileLoader<T, DP, 32, 64, DMA> Loader;
   constexpr uint32_t kTile = (uint32_t)Loader::kBytes;
@@ -270,30 +265,25 @@ __global__ __launch_bounds__(kThreads, 1) void few_kernel(const FwArgs<T> a) {
   const uint32_t token0 = behind ? a.seq.q_total : e.q_start;
   const size_t sample = behind ? 0 : e.sample;
   const uint32_t tokens = behind ? a.seq.tq - a.seq.q_total : a.seq.packed ? e.q_len : a.seq.tq;
-  const int64_t r0 = (int64_t)at.t * BM, rows = min((int64_t)tokens * sh.g - r0, (int64_t)BM);
-  if (rows <= 0) return;
-  const int lq = behind ? 0 : (int)e.q_len, lk = (int)e.k_len;
+  if ((uint64_t)at.t * BM >= (uint64_t)tokens * sh.g) return;
+  const int lq = behind ? 0 : (int)e.q_len, lk = (int)e.k_len, g = (int)sh.g;
+  const int r0 = (int)at.t * BM, rows = min((int)(tokens * sh.g) - r0, BM), filled = min(lq * g - r0, BM);
 
-  const int64_t r = r0 + (lane & 31);
-  const uint32_t tok = (uint32_t)(r / sh.g);
-  const bool exists = tok < tokens, valid = exists && (int)tok < lq;
-  const int lim = !valid ? 0 : sh.causal ? min(lk, max(0, (int)tok + lk - lq + 1)) : lk;
-  const int64_t last = min((int64_t)lq * sh.g, r0 + BM) - 1;
-  const int keys = last < r0 ? 0 : sh.causal ? min(lk, max(0, (int)(last / sh.g) + lk - lq + 1)) : lk;
-  const int all = last < r0 || last < r0 + BM - 1 ? 0 : sh.causal ? min(lk, max(0, (int)(r0 / sh.g) + lk - lq + 1)) : lk;
+  // the lane's row; keys that it, any row and all rows of the tile see
+  auto seen_by = [&](int rr) { return sh.causal ? min(lk, max(0, rr / g + lk - lq + 1)) : lk; };
+  const bool exists = (lane & 31) < rows, valid = (lane & 31) < filled;
+  const int lim = valid ? seen_by(r0 + (lane & 31)) : 0;
+  const int keys = filled <= 0 ? 0 : seen_by(r0 + filled - 1), all = filled < BM ? 0 : seen_by(r0);
   const uint32_t ranges = max(1u, ((uint32_t)keys + a.chunk - 1) / a.chunk);
   if (range >= ranges) return;
   const int from = (int)(range * a.chunk), to = min(keys, from + (int)a.chunk);
 
-  auto row_of = [&](int64_t rr) {
-    return (sample * a.seq.tq + token0 + (uint32_t)(rr / sh.g)) * sh.hq + head * sh.g + (uint32_t)(rr % sh.g);
-  };
+  const RowWalk walk((uint32_t)r0, sh);
+  const size_t row_base = (sample * a.seq.tq + token0) * sh.hq + head * sh.g;
   Frag<T> qf[DP / 16];
   {
-    const size_t row = row_of(exists ? r : r0);
-#pragma unroll
-    for (int c = 0; c < DP / 16; ++c)
-      qf[c] = load_frag(a.q + row * sh.d, valid, 16 * c + 8 * (lane >> 5), (int)sh.d, (Frag<T> *)nullptr);
+    const size_t row = row_base + walk.at(exists ? lane & 31 : 0, sh.hq);
+  load_row<T>(qf, a.q + row * sh.d, valid, sh, lane);
   }
   Rows<DP> st;
   reset(st);
@@ -309,7 +299,7 @@ __global__ __launch_bounds__(kThreads, 1) void few_kernel(const FwArgs<T> a) {
   auto fetch_v = [&](int key, int s) {
     lv_.fetch(vp + (size_t)min(key, to) * stride, to - key, 0, 1, 0, stride, 0, (int)sh.d, ring + (uint32_t)s * 2 * kTile + kTile, lane);
   };
-  constexpr int kStep = 32 * kWaves;
+  constexpr int kStep = 32 * W;
   int key = from + 32 * wave;
   if constexpr (DMA) {
     // blocks past the end are ordered too (they read nothing and write zeros), so that the waits count the same
@@ -319,9 +309,11 @@ __global__ __launch_bounds__(kThreads, 1) void few_kernel(const FwArgs<T> a) {
       fetch_k(key + s * kStep, s);
       fetch_v(key + s * kStep, s);
     }
+    arrived(qf);
     for (int s = 0; key < to; key += kStep, s = s + 1 == S ? 0 : s + 1) {
       const uint32_t stage = ring + (uint32_t)s * 2 * kTile;
       wait_loads<kInFlight>();
+      if (!sh.whole) Loader::clean(stage, (int)sh.d, lane);
       Scores<1> sc;
       scores<T, DP, 1>(sc, qf, stage + row_at);
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the block's reads are done before its place is filled again
@@ -352,6 +344,14 @@ __global__ __launch_bounds__(kThreads, 1) void few_kernel(const FwArgs<T> a) {
     }
   }
 
+  if constexpr (W == 1) {  // nothing to merge (the keys are not divided either): as the kernel for many rows
+    const float l = halves_sum(st.l);
+    if (!exists) return;
+    const size_t row = row_base + walk.at(lane & 31, sh.hq);
+    store_row<T, DP>(a.y + row * sh.d, st.o, 1.f / l, valid && l != 0.f, sh.d, a.vec_y != 0, lane);
+    if (a.stats != nullptr && lane < 32) a.stats[row] = !valid || l == 0.f ? -INFINITY : fmaf(st.m, sh.scale, logf(l));
+    return;
+  }
   // the wavefronts' results: per wavefront DP columns of 33 floats (rows across), then 32 maxima and 32 sums
   __syncthreads();
   float *const area = reinterpret_cast<float *>(lds);
@@ -371,40 +371,49 @@ __global__ __launch_bounds__(kThreads, 1) void few_kernel(const FwArgs<T> a) {
   __syncthreads();
   const bool whole = ranges == 1;
   const uint32_t tile = slot * sh.hk + head;
-  float *const part = a.partial + ((size_t)tile * a.splits + range) * (size_t)(BM * (DP + 2));
-  auto finish = [&](int row, uint32_t dd, float o, float m, float l) {
-    const size_t at_row = row_of(r0 + row);
-    a.y[at_row * sh.d + dd] = from_f32<T>(l == 0.f ? 0.f : o / l);
+  float *const part = a.partial + ((size_t)tile * a.splits + range) * (size_t)(BM * (DP + 4));
+  // four elements of a row
+  auto finish = [&](int row, uint32_t dd, const float (&o)[4], float m, float l) {
+    const size_t at_row = row_base + walk.at((uint32_t)row, sh.hq);
+    const float f = l == 0.f ? 0.f : 1.f / l;
+    const float four[4] = {o[0] * f, o[1] * f, o[2] * f, o[3] * f};
+    if (dd < sh.d) store4<T, false>(a.y + at_row * sh.d + dd, four, (int)(sh.d - dd), a.vec_y != 0);
     if (dd == 0 && a.stats != nullptr) a.stats[at_row] = l == 0.f ? -INFINITY : fmaf(m, sh.scale, logf(l));
   };
-  for (uint32_t i = tid; i < (uint32_t)rows * DP; i += kThreads) {
-    const int row = (int)(i / DP);
-    const uint32_t dd = i % DP;
+  for (uint32_t i = tid; i < (uint32_t)rows * (DP / 4); i += kThreads) {
+    const int row = (int)(i / (DP / 4));
+    const uint32_t dd = i % (DP / 4) * 4;
     float m = -INFINITY;
 #pragma unroll
-    for (int w = 0; w < kWaves; ++w) m = fmaxf(m, area[w * kPer + DP * 33 + row]);
+    for (int w = 0; w < W; ++w) m = fmaxf(m, area[w * kPer + DP * 33 + row]);
     const float base = m == -INFINITY ? 0.f : m * sh.scale_log2;
-    float l = 0.f, o = 0.f;
+    float l = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int w = 0; w < kWaves; ++w) {
+    for (int w = 0; w < W; ++w) {
       const float *his = area + w * kPer;
       const float lw = his[DP * 33 + 32 + row];
-      if (lw == 0.f) continue;  // it has seen no key of this row
-      const float f = exp2_fast(fmaf(his[DP * 33 + row], sh.scale_log2, -base));
+      // a wavefront that has seen no key of this row has a sum of 0 and its rows are 0
+      const float f = lw == 0.f ? 0.f : exp2_fast(fmaf(his[DP * 33 + row], sh.scale_log2, -base));
       l = fmaf(lw, f, l);
-      o = fmaf(his[dd * 33 + row], f, o);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[e] = lw == 0.f ? o[e] : fmaf(his[(dd + e) * 33 + row], f, o[e]);
     }
     if (whole) {
-      if (dd < sh.d) finish(row, dd, o, m, l);
+      finish(row, dd, o, m, l);
     } else {
-      store_shared(part + row * (DP + 2) + dd, o);
-      if (dd < 2) store_shared(part + row * (DP + 2) + DP + dd, dd == 0 ? m : l);
+      float *p = part + row * (DP + 4);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) store_shared(p + dd + e, o[e]);
+      if (dd == 0) {
+        store_shared(p + DP, m);
+        store_shared(p + DP + 1, l);
+      }
     }
   }
   if (whole || !last_of_tile(a.tickets + tile, ranges, &flag)) return;
-  // The last of the tile: each thread has one element of a row at a time and takes the ranges 16 at a time, all their
+  // The last of the tile: each thread has an element of a row at a time and takes the ranges 16 at a time, all their
   // loads in flight together.
-  const float *const all_parts = a.partial + (size_t)tile * a.splits * (size_t)(BM * (DP + 2));
+  const float *const all_parts = a.partial + (size_t)tile * a.splits * (size_t)(BM * (DP + 4));
   for (uint32_t i = tid; i < (uint32_t)rows * DP; i += kThreads) {
     const int row = (int)(i / DP);
     const uint32_t dd = i % DP;
@@ -413,7 +422,7 @@ __global__ __launch_bounds__(kThreads, 1) void few_kernel(const FwArgs<T> a) {
       float pm[16], pl[16], po[16];
 #pragma unroll
       for (uint32_t u = 0; u < 16; ++u) {
-        const float *p = all_parts + (size_t)min(p0 + u, ranges - 1) * (BM * (DP + 2)) + row * (DP + 2);
+        const float *p = all_parts + (size_t)min(p0 + u, ranges - 1) * (BM * (DP + 4)) + row * (DP + 4);
         pm[u] = load_shared(p + DP);
         pl[u] = load_shared(p + DP + 1);
         po[u] = load_shared(p + dd);
@@ -428,13 +437,16 @@ __global__ __launch_bounds__(kThreads, 1) void few_kernel(const FwArgs<T> a) {
       m = top;
 #pragma unroll
       for (uint32_t u = 0; u < 16; ++u) {
-        const float fu = p0 + u >= ranges || pl[u] == 0.f ? 0.f : exp2_fast(fmaf(pm[u], sh.scale_log2, -base));
-        if (fu == 0.f) continue;
-        l = fmaf(pl[u], fu, l);
-        o = fmaf(po[u], fu, o);
+        const bool none = p0 + u >= ranges || pl[u] == 0.f;
+        const float fu = none ? 0.f : exp2_fast(fmaf(pm[u], sh.scale_log2, -base));
+        l = none ? l : fmaf(pl[u], fu, l);
+        o = none ? o : fmaf(po[u], fu, o);
       }
     }
-    if (dd < sh.d) finish(row, dd, o, m, l);
+    if (dd >= sh.d) continue;
+    const size_t at_row = row_base + walk.at((uint32_t)row, sh.hq);
+    a.y[at_row * sh.d + dd] = from_f32<T>(l == 0.f ? 0.f : o / l);
+    if (dd == 0 && a.stats != nullptr) a.stats[at_row] = l == 0.f ? -INFINITY : fmaf(m, sh.scale, logf(l));
   }
 }
 
@@ -452,38 +464,37 @@ int launch_rows(phip_ctx *ctx, FwArgs<T> a) {
   return PHIP_OK;
 }
 
-// Keys per range of the kernel for few rows.  One workgroup fits on a CU (its ring of tiles), so the time is about the
-// keys of a range times the rounds that the ranges take on the chip: the shortest range that fills it once, or, when
-// there are more tiles than that, ranges of a quarter of the average, which even out different lengths.
-uint32_t few_chunk(phip_ctx *ctx, const SequenceView &view, const phip_sequences *seqs, const Shape &s, uint64_t tiles) {
+// Keys per range of the kernel for few rows.  One workgroup of four wavefronts fits on a CU (its ring of tiles), so the
+// time is about the keys of a range times the rounds that the ranges take on the chip: ranges that fill it about once.
+uint32_t few_chunk(phip_ctx *ctx, const SequenceView &view, const phip_sequences *seqs, uint64_t tiles) {
   const uint64_t cus = (uint64_t)ctx->prop.multiProcessorCount;
   const uint64_t most = seqs != nullptr ? seqs->max_k : view.tk;
-  if (tiles > (uint64_t)kTicketSlots) return (uint32_t)most + 1;
-  const uint64_t keys = (seqs != nullptr ? seqs->k_sum : (uint64_t)view.n * view.tk) * s.hk;
-  uint64_t chunk = (keys + cus - 1) / cus;
+  if (tiles >= cus || tiles > (uint64_t)kTicketSlots) return (uint32_t)most + 1;
+  const uint64_t sum = seqs != nullptr ? seqs->k_sum : (uint64_t)view.n * view.tk;
+  uint64_t chunk = sum * tiles / view.n / cus;
   if (chunk < 256) chunk = 256;
   return (uint32_t)std::min<uint64_t>((chunk + 127) / 128 * 128, 1u << 30);
 }
 
-template <typename T, int DP, bool DMA>
+template <typename T, int DP, bool DMA, int W>
 int launch_few(phip_ctx *ctx, FwArgs<T> a, const phip_sequences *seqs) {
-  constexpr int lds = kFewLds<T, DP>;
-  const int rc = allow_lds<few_kernel<T, DP, DMA>>(ctx, lds);
+  constexpr int lds = kFewLds<T, DP, W>;
+  const int rc = allow_lds<few_kernel<T, DP, DMA, W>>(ctx, lds);
   if (rc != PHIP_OK) return rc;
   a.tiles = (uint32_t)(((uint64_t)a.seq.tq * a.s.g + 31) / 32);
   const uint64_t tiles = slots(a.seq, 32, a.s.g, false) * a.s.hk;
-  a.chunk = few_chunk(ctx, a.seq, seqs, a.s, tiles);
   const uint32_t most = seqs != nullptr ? seqs->max_k : a.seq.tk;
+  a.chunk = W == 1 ? most + 1 : few_chunk(ctx, a.seq, seqs, tiles);
   a.splits = most <= a.chunk ? 1 : (most + a.chunk - 1) / a.chunk;
   PHIP_REQUIRE(tiles * a.splits < 0x7fffffffu, "too many rows");
   void *partial = nullptr;
   if (a.splits > 1) {
-    const int rc2 = phip_pool_alloc(ctx, (size_t)tiles * a.splits * 32 * (DP + 2) * sizeof(float), &partial, nullptr);
+    const int rc2 = phip_pool_alloc(ctx, (size_t)tiles * a.splits * 32 * (DP + 4) * sizeof(float), &partial, nullptr);
     if (rc2 != PHIP_OK) return rc2;
     a.partial = static_cast<float *>(partial);
     a.tickets = tile_tickets(ctx);
   }
-  hipLaunchKernelGGL((few_kernel<T, DP, DMA>), dim3((uint32_t)(tiles * a.splits)), dim3(kThreads), lds, ctx->stream, a);
+  hipLaunchKernelGGL((few_kernel<T, DP, DMA, W>), dim3((uint32_t)(tiles * a.splits)), dim3(64 * W), lds, ctx->stream, a);
   const hipError_t e = hipGetLastError();
   if (partial != nullptr) phip_pool_free(ctx, partial);
   if (e != hipSuccess) return fail(PHIP_ERR_RUNTIME, "launching the attention kernel failed: %s", hipGetErrorString(e));
@@ -492,8 +503,12 @@ int launch_few(phip_ctx *ctx, FwArgs<T> a, const phip_sequences *seqs) {
 
 template <typename T, int DP>
 int launch(phip_ctx *ctx, const FwArgs<T> &a, const phip_sequences *seqs, bool dma) {
-  const uint32_t most = seqs != nullptr ? seqs->max_q : a.seq.tq;
-  if ((uint64_t)most * a.s.g <= 32) return dma ? launch_few<T, DP, true>(ctx, a, seqs) : launch_few<T, DP, false>(ctx, a, seqs);
+  const uint64_t wide = slots(a.seq, 128, a.s.g, false) * a.s.hk, narrow = slots(a.seq, 32, a.s.g, false) * a.s.hk;
+  const uint64_t most = (uint64_t)(seqs != nullptr ? seqs->max_q : a.seq.tq) * a.s.g;
+  Way way = choose_way<T>(ctx, wide, narrow, most, seqs != nullptr ? seqs->max_k : a.seq.tk);
+  if (way == Way::Shared && most <= 32) way = Way::Four;
+  if (way == Way::One) return dma ? launch_few<T, DP, true, 1>(ctx, a, seqs) : launch_few<T, DP, false, 1>(ctx, a, seqs);
+  if (way == Way::Four) return dma ? launch_few<T, DP, true, 4>(ctx, a, seqs) : launch_few<T, DP, false, 4>(ctx, a, seqs);
   return dma ? launch_rows<T, DP, true>(ctx, a) : launch_rows<T, DP, false>(ctx, a);
 }
 
@@ -516,7 +531,8 @@ int forward(phip_ctx *ctx, const T *q, const T *k, const T *v, T *y, float *stat
   a.y = y;
   a.stats = stats;
   a.vec_y = d % 4 == 0 && reinterpret_cast<uintptr_t>(y) % (4 * sizeof(T)) == 0;
-  const bool dma = rows_movable(d, sizeof(T), {k, v});
+  a.s.whole = rows_aligned(d, sizeof(T), 16, {q, k, v});
+  const bool dma = rows_aligned(d, sizeof(T), 4, {q, k, v});
   switch ((d + 31) / 32) {
     case 1: return launch<T, 32>(ctx, a, seqs, dma);
     case 2: return launch<T, 64>(ctx, a, seqs, dma);
