@@ -329,7 +329,22 @@ struct TileLoader {
   static constexpr int kBytes = ROWS * L::kPitch;
   static constexpr int kInstr = kBytes / 16 / NT;
   static_assert(kBytes % (16 * NT) == 0, "a tile is a whole number of chunks per thread");
+  static constexpr int kRowsPer = NT / L::kChunks;  // rows that one load per thread covers
   u32x4 held[DMA ? 1 : kInstr];
+  // Load q of a thread takes row q kRowsPer + lane_row of the tile.  The swizzle is linear over the bits of the row, so the
+  // thread's chunk is the one of its first row, exclusive-or a constant of q; and with g a divisor of kRowsPer the rows of q
+  // lie `step` bytes behind each other.  So three registers describe a thread's part of every tile.
+  uint32_t rowpart, c16, step;
+  int lane_row;
+  bool linear;
+
+  __device__ inline void init(uint32_t g, uint32_t stride, uint32_t inner, int tid) {
+    lane_row = tid / L::kChunks;
+    c16 = (uint32_t)(((tid % L::kChunks) ^ L::swizzle(lane_row)) << 4);
+    linear = kRowsPer % g == 0;
+    rowpart = ((uint32_t)lane_row / g * stride + (uint32_t)lane_row % g * inner) * (uint32_t)sizeof(T);
+    step = kRowsPer / g * stride * (uint32_t)sizeof(T);
+  }
 
   // rows_left: rows of the tile that exist (may be <= 0 or more than ROWS).  first: where the tile's first row lies in
   // its group of g (0 when g == 1); base is the address of row -first (any address when no row exists).
@@ -338,26 +353,36 @@ struct TileLoader {
     if constexpr (DMA) {
       uint32_t bytes = 0x7fffffffu;
       if (d % L::kPerChunk != 0) {  // the buffer ends with the last row that exists: nothing behind it is read
-        const uint32_t last = first + (uint32_t)max(0, min(rows_left, ROWS) - 1), t = g == 1 ? last : (last * inv_g) >> 22;
+        const uint32_t last = first + (uint32_t)max(0, min(rows_left, ROWS) - 1), t = (last * inv_g) >> 22;
         bytes = rows_left > 0 ? (t * stride + (last - t * g) * inner + (uint32_t)d) * (uint32_t)sizeof(T) : 0;
       }
       const u32x4 rsrc = buffer_words(base, bytes);
       const uint32_t wave_at = (uint32_t)__builtin_amdgcn_readfirstlane((tid & ~63) * 16);
+      const uint32_t row_bytes = (uint32_t)d * (uint32_t)sizeof(T);
+      if (linear) {
 #pragma unroll
-      for (int q = 0; q < kInstr; ++q) {
-        const int slot = q * NT + tid;
-        uint32_t off;
-        const bool in = place(slot, rows_left, first, g, inv_g, stride, inner, d, &off);
-        lds_dma_b128(rsrc, lds_addr + wave_at + (uint32_t)(q * NT * 16), in ? off * (uint32_t)sizeof(T) : kOutOfRange);
+        for (int q = 0; q < kInstr; ++q) {
+          const uint32_t c = c16 ^ (uint32_t)(L::swizzle(q * kRowsPer) << 4), off = rowpart + c + (uint32_t)q * step;
+          const bool in = lane_row < rows_left - q * kRowsPer && c < row_bytes;
+          lds_dma_b128(rsrc, lds_addr + wave_at + (uint32_t)(q * NT * 16), in ? off : kOutOfRange);
+        }
+      } else {
+#pragma unroll
+        for (int q = 0; q < kInstr; ++q) {
+          const uint32_t c = c16 ^ (uint32_t)(L::swizzle(q * kRowsPer) << 4);
+          const uint32_t r = first + (uint32_t)(lane_row + q * kRowsPer), t = (r * inv_g) >> 22;
+          const uint32_t off = (t * stride + (r - t * g) * inner) * (uint32_t)sizeof(T) + c;
+          const bool in = lane_row < rows_left - q * kRowsPer && c < row_bytes;
+          lds_dma_b128(rsrc, lds_addr + wave_at + (uint32_t)(q * NT * 16), in ? off : kOutOfRange);
+        }
       }
     } else {
 #pragma unroll
       for (int q = 0; q < kInstr; ++q) {
-        uint32_t off;
-        const int slot = q * NT + tid;
-        const bool in = place(slot, rows_left, first, g, inv_g, stride, inner, d, &off);
-        const int c0 = ((slot % L::kChunks) ^ L::swizzle(slot / L::kChunks)) * L::kPerChunk;
-        held[q] = load_part<false, DP == 32>(base + (in ? off - (uint32_t)c0 : 0), in, c0, d);
+        const int c0 = (int)(c16 ^ (uint32_t)(L::swizzle(q * kRowsPer) << 4)) / (int)sizeof(T);
+        const uint32_t r = first + (uint32_t)(lane_row + q * kRowsPer), t = (r * inv_g) >> 22;
+        const bool in = lane_row + q * kRowsPer < rows_left && c0 < d;
+        held[q] = load_part<false, DP == 32>(base + (in ? t * stride + (r - t * g) * inner : 0), in, c0, d);
       }
     }
   }
@@ -377,20 +402,6 @@ struct TileLoader {
       for (int w = 0; w < 4; ++w)  // rows are whole dwords
         if (w * 4 >= d % L::kPerChunk * (int)sizeof(T)) *lds_ptr<uint32_t>(chunk + 4 * w) = 0;
     }
-  }
-
- private:
-  // Element offset of the chunk that belongs at position `slot` of the tile; false where nothing lies there.
-  __device__ static inline bool place(int slot, int rows_left, uint32_t first, uint32_t g, uint32_t inv_g, uint32_t stride,
-                                      uint32_t inner, int d, uint32_t *off) {
-    const int row = slot / L::kChunks, c = (slot % L::kChunks) ^ L::swizzle(row);
-    if (g == 1) {
-      *off = (uint32_t)row * stride + (uint32_t)(c * L::kPerChunk);
-    } else {
-      const uint32_t r = first + (uint32_t)row, t = (r * inv_g) >> 22;
-      *off = t * stride + (r - t * g) * inner + (uint32_t)(c * L::kPerChunk);
-    }
-    return row < rows_left && c * L::kPerChunk < d;
   }
 };
 
@@ -560,6 +571,12 @@ inline bool rows_aligned(uint32_t d, size_t item, size_t unit, std::initializer_
   if (d * item % unit != 0) return false;
   for (const void *p : ptrs)
     if (reinterpret_cast<uintptr_t>(p) % unit != 0) return false;
+  return true;
+}
+
+inline bool elements_aligned(size_t item, std::initializer_list<const void *> ptrs) {
+  for (const void *p : ptrs)
+    if (reinterpret_cast<uintptr_t>(p) % item != 0) return false;
   return true;
 }
 

@@ -112,11 +112,13 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void queries_kern
   const T *vp = a.v + ((sample * a.seq.tk + e.k_start) * sh.hk + head) * (size_t)sh.d;
   const uint32_t row_at = L::row_lane(lane), col_at = L::col_lane(lane);
   Loader lk_, lv_;
+  lk_.init(1, stride, 0, tid);
+  lv_ = lk_;
   auto fetch = [&](int t) {
     const uint32_t stage = lds0 + (uint32_t)(t & 1) * 2 * kTile;
     const size_t off = (size_t)t * KT * stride;
-    lk_.fetch(kp + off, lk - t * KT, 0, 1, 0, stride, 0, (int)sh.d, stage, tid);
-    lv_.fetch(vp + off, lk - t * KT, 0, 1, 0, stride, 0, (int)sh.d, stage + kTile, tid);
+    lk_.fetch(kp + off, lk - t * KT, 0, 1, 1u << 22, stride, 0, (int)sh.d, stage, tid);
+    lv_.fetch(vp + off, lk - t * KT, 0, 1, 1u << 22, stride, 0, (int)sh.d, stage + kTile, tid);
   };
   const int n = (wg_keys + KT - 1) / KT;
   if (n > 0) fetch(0);
@@ -139,17 +141,20 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void queries_kern
     const bool masked = (t + 1) * KT > w_all;
 #pragma unroll
     for (int kb = 0; kb < KT / 32; ++kb) {
+      __builtin_amdgcn_sched_barrier(0);
       f32x16 p = f32x16{}, dp = f32x16{};
 #pragma unroll
       for (int c = 0; c < DP / 16; ++c) mma(p, L::row_frag(stage + row_at, kb, c), qf[c]);
 #pragma unroll
       for (int c = 0; c < DP / 16; ++c) mma(dp, L::row_frag(stage + kTile + row_at, kb, c), gf[c]);
+      __builtin_amdgcn_sched_barrier(0);
       const int first = t * KT + 32 * kb + 4 * (lane >> 5);
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
         const float x = exp2_fast(fmaf(p[i], sh.scale_log2, -base)) * (dp[i] - delta);
         p[i] = masked && first + block_row(i) >= lim ? 0.f : x;
       }
+      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
         const Frag<T> ds = as_operand(p, c, (Frag<T> *)nullptr);
@@ -171,9 +176,11 @@ __device__ inline void keys_block(f32x16 (&gk)[DP / 32], f32x16 (&gv)[DP / 32], 
   const uint32_t g_at = q_at + to_g;
   in += (uint32_t)(4 * (lane >> 5) * 8);
   hidden -= 4 * (lane >> 5);
+  __builtin_amdgcn_sched_barrier(0);
   f32x16 p = f32x16{};
 #pragma unroll
   for (int c = 0; c < DP / 16; ++c) mma(p, L::row_frag(q_at + row_at, 0, c), kf[c]);
+  __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
   for (int i2 = 0; i2 < 8; ++i2) {
     const f32x4 pair = *lds_ptr<f32x4>(in + (uint32_t)(block_row(2 * i2) * 8));  // two rows: base, delta, base, delta
@@ -184,15 +191,18 @@ __device__ inline void keys_block(f32x16 (&gk)[DP / 32], f32x16 (&gv)[DP / 32], 
       if (masked && block_row(i) < hidden) p[i] = 0.f;
     }
   }
+  __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
   for (int c = 0; c < 2; ++c) {
     const Frag<T> pf = as_operand(p, c, (Frag<T> *)nullptr);
 #pragma unroll
     for (int db = 0; db < DP / 32; ++db) mma(gv[db], L::col_frag(g_at + col_at, c, db), pf);
   }
+  __builtin_amdgcn_sched_barrier(0);
   f32x16 dp = f32x16{};
 #pragma unroll
   for (int c = 0; c < DP / 16; ++c) mma(dp, L::row_frag(g_at + row_at, 0, c), vf[c]);
+  __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
   for (int i2 = 0; i2 < 8; ++i2) {
     const f32x4 pair = *lds_ptr<f32x4>(in + (uint32_t)(block_row(2 * i2) * 8));
@@ -202,6 +212,7 @@ __device__ inline void keys_block(f32x16 (&gk)[DP / 32], f32x16 (&gv)[DP / 32], 
       dp[i] = p[i] == 0.f ? 0.f : p[i] * (dp[i] - pair[2 * e + 1]);
     }
   }
+  __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
   for (int c = 0; c < 2; ++c) {
     const Frag<T> ds = as_operand(dp, c, (Frag<T> *)nullptr);
@@ -257,6 +268,8 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 && DMA ? 2 : 1) void keys_
   const T *qp = a.q + q_row0 * sh.d, *gp = a.gy + q_row0 * sh.d;
   const uint32_t row_at = L::row_lane(lane), col_at = L::col_lane(lane);
   Loader lq_, lg_;
+  lq_.init(sh.g, sh.hq * sh.d, sh.d, tid);
+  lg_ = lq_;
   RowWalk walk((uint32_t)wg_first, sh);
   float value = 0.f;
   // the tile of rows from r on, where the walk stands, into a stage; the values of a row side by side
@@ -267,10 +280,12 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 && DMA ? 2 : 1) void keys_
     lq_.fetch(qp + off, left, walk.in0, sh.g, sh.inv_g, sh.hq * sh.d, sh.d, (int)sh.d, stage, tid);
     lg_.fetch(gp + off, left, walk.in0, sh.g, sh.inv_g, sh.hq * sh.d, sh.d, (int)sh.d, stage + kTile, tid);
     // rows past the end get zeros, which with their zeros for q and gy add nothing
-    const bool in = (tid >> 1) < left;
+    int lane_id = tid;
+    asm volatile("" : "+v"(lane_id));
+    const bool in = (lane_id >> 1) < left;
     const float *p = reinterpret_cast<const float *>(a.values + q_row0 + (size_t)walk.t0 * sh.hq);
-    const uint32_t rr = walk.in0 + ((uint32_t)tid >> 1), t = (rr * sh.inv_g) >> 22;
-    const uint32_t at_value = 2 * (t * sh.hq + (rr - t * sh.g)) + (tid & 1);
+    const uint32_t rr = walk.in0 + ((uint32_t)lane_id >> 1), t = (rr * sh.inv_g) >> 22;
+    const uint32_t at_value = 2 * (t * sh.hq + (rr - t * sh.g)) + (lane_id & 1);
     if (wave < 2 * QT / 64) {
       if constexpr (DMA)
         lds_dma_b32(buffer_words(p, 0x7fffffffu), values0 + (uint32_t)((stage_no * 2 * QT + wave * 64) * 4), in ? at_value * 4 : kOutOfRange);
@@ -396,10 +411,12 @@ __global__ __launch_bounds__(64 * W, 1) void few_queries_kernel(const BwArgs<T> 
   const uint32_t row_at = L::row_lane(lane), col_at = L::col_lane(lane);
   constexpr int kStep = 32 * W;
   Loader lk_, lv_;
+  lk_.init(1, stride, 0, lane);
+  lv_ = lk_;
   auto fetch = [&](int key, int s) {
     const size_t off = (size_t)min(key, keys) * stride;
-    lk_.fetch(kp + off, keys - key, 0, 1, 0, stride, 0, (int)sh.d, ring + (uint32_t)s * 2 * kTile, lane);
-    lv_.fetch(vp + off, keys - key, 0, 1, 0, stride, 0, (int)sh.d, ring + (uint32_t)s * 2 * kTile + kTile, lane);
+    lk_.fetch(kp + off, keys - key, 0, 1, 1u << 22, stride, 0, (int)sh.d, ring + (uint32_t)s * 2 * kTile, lane);
+    lv_.fetch(vp + off, keys - key, 0, 1, 1u << 22, stride, 0, (int)sh.d, ring + (uint32_t)s * 2 * kTile + kTile, lane);
   };
   Frag<T> qf[DP / 16], gf[DP / 16];
   float delta = 0.f;
@@ -503,6 +520,8 @@ __global__ __launch_bounds__(64 * W, 1) void few_keys_kernel(const BwArgs<T> a) 
   const uint32_t row_at = L::row_lane(lane), col_at = L::col_lane(lane);
   constexpr int kStep = 32 * W;
   Loader lq_, lg_;
+  lq_.init(sh.g, sh.hq * sh.d, sh.d, lane);
+  lg_ = lq_;
   float value = 0.f;
   int rr = first_row(k0) / 32 * 32 + 32 * wave;
   RowWalk walk((uint32_t)rr, sh);
@@ -591,13 +610,13 @@ int launch(phip_ctx *ctx, BwArgs<T> a, const phip_sequences *seqs) {
                               : launch_kernel<few_keys_kernel<T, DP, DMA, 1>>(ctx, a, narrow_k, 64, kFewLds<T, DP, 1>);
 }
 
-template <typename T>
-int dispatch(phip_ctx *ctx, const BwArgs<T> &a, const phip_sequences *seqs, bool dma) {
+template <typename T, bool DMA>
+int dispatch(phip_ctx *ctx, const BwArgs<T> &a, const phip_sequences *seqs) {
   switch ((a.s.d + 31) / 32) {
-    case 1: return dma ? launch<T, 32, true>(ctx, a, seqs) : launch<T, 32, false>(ctx, a, seqs);
-    case 2: return dma ? launch<T, 64, true>(ctx, a, seqs) : launch<T, 64, false>(ctx, a, seqs);
-    case 3: return dma ? launch<T, 96, true>(ctx, a, seqs) : launch<T, 96, false>(ctx, a, seqs);
-    default: return dma ? launch<T, 128, true>(ctx, a, seqs) : launch<T, 128, false>(ctx, a, seqs);
+    case 1: return launch<T, 32, DMA>(ctx, a, seqs);
+    case 2: return launch<T, 64, DMA>(ctx, a, seqs);
+    case 3: return launch<T, 96, DMA>(ctx, a, seqs);
+    default: return launch<T, 128, DMA>(ctx, a, seqs);
   }
 }
 
@@ -612,6 +631,8 @@ int backward(phip_ctx *ctx, const T *q, const T *k, const T *v, const T *y, cons
   rc = sequence_view(ctx, seqs, tq, tk, bs, true, &a.seq);
   if (rc != PHIP_OK) return rc;
   PHIP_REQUIRE(q && k && v && y && stats && gy && gq && gk && gv, "null pointer");
+  PHIP_REQUIRE(elements_aligned(sizeof(T), {q, k, v, y, gy, gq, gk, gv}) && elements_aligned(4, {stats}),
+               "an address is no multiple of the element size");
   const size_t nq = (size_t)d * hq * tq * bs * sizeof(T), nk = (size_t)d * hk * tk * bs * sizeof(T);
   const size_t ns = (size_t)hq * tq * bs * sizeof(float);
   auto is_read = [&](const void *g, size_t n) {
@@ -647,7 +668,13 @@ int backward(phip_ctx *ctx, const T *q, const T *k, const T *v, const T *y, cons
   auto vec = [&](const void *p) { return reinterpret_cast<uintptr_t>(p) % (4 * sizeof(T)) == 0; };
   a.vec = d % 4 == 0 && vec(gq) && vec(gk) && vec(gv);
   a.s.whole = rows_aligned(d, sizeof(T), 16, {q, k, v, y, gy});
-  rc = dispatch<T>(ctx, a, seqs, rows_aligned(d, sizeof(T), 4, {q, k, v, y, gy}));
+  // fp32 rows are always whole dwords; 16-bit rows of an odd size are not
+  bool dma = true;
+  if constexpr (sizeof(T) == 2) {
+    dma = rows_aligned(d, sizeof(T), 4, {q, k, v, gy});
+    if (!dma) rc = dispatch<T, false>(ctx, a, seqs);
+  }
+  if (dma) rc = dispatch<T, true>(ctx, a, seqs);
   phip_pool_free(ctx, values);
   return rc;
 }

@@ -175,11 +175,13 @@ __global__ __launch_bounds__(kThreads, 2) void rows_kernel(const FwArgs<T> a) {
   const T *vp = a.v + ((sample * a.seq.tk + e.k_start) * sh.hk + head) * (size_t)sh.d;
   const uint32_t row_at = L::row_lane(lane), col_at = L::col_lane(lane);
   Loader lk_, lv_;
+  lk_.init(1, stride, 0, tid);
+  lv_ = lk_;
   auto fetch = [&](int t) {
     const uint32_t stage = lds0 + (uint32_t)(t & 1) * 2 * kTile;
     const size_t off = (size_t)t * KT * stride;
-    lk_.fetch(kp + off, lk - t * KT, 0, 1, 0, stride, 0, (int)sh.d, stage, tid);
-    lv_.fetch(vp + off, lk - t * KT, 0, 1, 0, stride, 0, (int)sh.d, stage + kTile, tid);
+    lk_.fetch(kp + off, lk - t * KT, 0, 1, 1u << 22, stride, 0, (int)sh.d, stage, tid);
+    lv_.fetch(vp + off, lk - t * KT, 0, 1, 1u << 22, stride, 0, (int)sh.d, stage + kTile, tid);
   };
   const int n = (wg_keys + KT - 1) / KT;
   if (n > 0) fetch(0);
@@ -293,11 +295,13 @@ __global__ __launch_bounds__(64 * W, 1) void few_kernel(const FwArgs<T> a) {
   const uint32_t ring = lds0 + (uint32_t)wave * (2 * S * kTile);
   const uint32_t row_at = L::row_lane(lane), col_at = L::col_lane(lane);
   Loader lk_, lv_;
+  lk_.init(1, stride, 0, lane);
+  lv_ = lk_;
   auto fetch_k = [&](int key, int s) {
-    lk_.fetch(kp + (size_t)min(key, to) * stride, to - key, 0, 1, 0, stride, 0, (int)sh.d, ring + (uint32_t)s * 2 * kTile, lane);
+    lk_.fetch(kp + (size_t)min(key, to) * stride, to - key, 0, 1, 1u << 22, stride, 0, (int)sh.d, ring + (uint32_t)s * 2 * kTile, lane);
   };
   auto fetch_v = [&](int key, int s) {
-    lv_.fetch(vp + (size_t)min(key, to) * stride, to - key, 0, 1, 0, stride, 0, (int)sh.d, ring + (uint32_t)s * 2 * kTile + kTile, lane);
+    lv_.fetch(vp + (size_t)min(key, to) * stride, to - key, 0, 1, 1u << 22, stride, 0, (int)sh.d, ring + (uint32_t)s * 2 * kTile + kTile, lane);
   };
   constexpr int kStep = 32 * W;
   int key = from + 32 * wave;
@@ -501,15 +505,25 @@ int launch_few(phip_ctx *ctx, FwArgs<T> a, const phip_sequences *seqs) {
   return PHIP_OK;
 }
 
-template <typename T, int DP>
-int launch(phip_ctx *ctx, const FwArgs<T> &a, const phip_sequences *seqs, bool dma) {
+template <typename T, int DP, bool DMA>
+int launch(phip_ctx *ctx, const FwArgs<T> &a, const phip_sequences *seqs) {
   const uint64_t wide = slots(a.seq, 128, a.s.g, false) * a.s.hk, narrow = slots(a.seq, 32, a.s.g, false) * a.s.hk;
   const uint64_t most = (uint64_t)(seqs != nullptr ? seqs->max_q : a.seq.tq) * a.s.g;
   Way way = choose_way<T>(ctx, wide, narrow, most, seqs != nullptr ? seqs->max_k : a.seq.tk);
   if (way == Way::Shared && most <= 32) way = Way::Four;
-  if (way == Way::One) return dma ? launch_few<T, DP, true, 1>(ctx, a, seqs) : launch_few<T, DP, false, 1>(ctx, a, seqs);
-  if (way == Way::Four) return dma ? launch_few<T, DP, true, 4>(ctx, a, seqs) : launch_few<T, DP, false, 4>(ctx, a, seqs);
-  return dma ? launch_rows<T, DP, true>(ctx, a) : launch_rows<T, DP, false>(ctx, a);
+  if (way == Way::One) return launch_few<T, DP, DMA, 1>(ctx, a, seqs);
+  if (way == Way::Four) return launch_few<T, DP, DMA, 4>(ctx, a, seqs);
+  return launch_rows<T, DP, DMA>(ctx, a);
+}
+
+template <typename T, bool DMA>
+int dispatch(phip_ctx *ctx, const FwArgs<T> &a, const phip_sequences *seqs) {
+  switch ((a.s.d + 31) / 32) {
+    case 1: return launch<T, 32, DMA>(ctx, a, seqs);
+    case 2: return launch<T, 64, DMA>(ctx, a, seqs);
+    case 3: return launch<T, 96, DMA>(ctx, a, seqs);
+    default: return launch<T, 128, DMA>(ctx, a, seqs);
+  }
 }
 
 template <typename T>
@@ -522,6 +536,7 @@ int forward(phip_ctx *ctx, const T *q, const T *k, const T *v, T *y, float *stat
   rc = sequence_view(ctx, seqs, tq, tk, bs, true, &a.seq);
   if (rc != PHIP_OK) return rc;
   PHIP_REQUIRE(q != nullptr && k != nullptr && v != nullptr && y != nullptr, "null pointer");
+  PHIP_REQUIRE(elements_aligned(sizeof(T), {q, k, v, y}), "an address is no multiple of the element size");
   const size_t ny = (size_t)d * hq * tq * bs * sizeof(T), nk = (size_t)d * hk * tk * bs * sizeof(T);
   PHIP_REQUIRE(!shares_memory(y, ny, q, ny) && !shares_memory(y, ny, k, nk) && !shares_memory(y, ny, v, nk),
                "the result shares memory with an operand");
@@ -532,13 +547,11 @@ int forward(phip_ctx *ctx, const T *q, const T *k, const T *v, T *y, float *stat
   a.stats = stats;
   a.vec_y = d % 4 == 0 && reinterpret_cast<uintptr_t>(y) % (4 * sizeof(T)) == 0;
   a.s.whole = rows_aligned(d, sizeof(T), 16, {q, k, v});
-  const bool dma = rows_aligned(d, sizeof(T), 4, {q, k, v});
-  switch ((d + 31) / 32) {
-    case 1: return launch<T, 32>(ctx, a, seqs, dma);
-    case 2: return launch<T, 64>(ctx, a, seqs, dma);
-    case 3: return launch<T, 96>(ctx, a, seqs, dma);
-    default: return launch<T, 128>(ctx, a, seqs, dma);
+  // fp32 rows are always whole dwords; 16-bit rows of an odd size are not
+  if constexpr (sizeof(T) == 2) {
+    if (!rows_aligned(d, sizeof(T), 4, {q, k, v})) return dispatch<T, false>(ctx, a, seqs);
   }
+  return dispatch<T, true>(ctx, a, seqs);
 }
 
 }  // namespace
