@@ -9,7 +9,7 @@
 // takes a few tokens with all their heads of queries and keys: the cosines and sines are the same for all heads, so they
 // are computed once per token into LDS.  A row is spread over the fewest lanes that hold it at two 16-byte chunks each, one
 // for either side of its pairs, so a pair never leaves its lane and the norm is a few exchanges between neighbours.
-#include <type_traits>
+#include <algorithm>
 
 #include "phip_pointwise.h"
 #include "phip_sequences.h"
@@ -23,21 +23,29 @@ using pointwise::kBlock;
 constexpr uint32_t kMostSize = 128;
 constexpr int kMostTokens = 8;   // per workgroup and step
 
+// One of the two tensors of a call: queries or keys.
+template <typename T>
+struct Side {
+  const T *x;             // forward: the operand; backward: the same (norm only)
+  const T *w;             // weights of the norm
+  const T *gy;            // backward
+  T *o;                   // y, or gx
+  uint32_t heads, inv;    // inv: ceil(2^32 / heads), 0 for one head
+  uint32_t acc;           // backward: add into what is there
+  uint32_t blocks;        // workgroups that have tokens (and, with weights, leave sums)
+  uint32_t tt;            // tokens per step of a workgroup
+};
+
 template <typename T>
 struct Args {
-  const T *xq, *xk;       // forward: the operands; backward: the same (norm only)
-  const T *wq, *wk;       // weights of the norm
-  const T *gyq, *gyk;     // backward
-  T *oq, *ok;             // y, or gx
-  float *partial;         // backward with weights: per workgroup, d sums for wq, then d for wk
+  Side<T> side[2];        // queries, keys; blockIdx.y tells which
+  float *partial;         // backward with weights: per workgroup of either side, d sums
   SequenceView seq;
   uint32_t tokens;        // tq * batch
-  uint32_t d, hq, h;      // h: heads of queries and keys together
-  uint32_t tt;            // tokens per step of a workgroup
+  uint32_t d;
   uint32_t pairs, items, lanes;  // items: lanes of a row that have work; lanes: the power of two that a row takes
   int32_t first;
   float amplitude, eps;
-  uint32_t acc_q, acc_k;  // backward: add into what is there
   float f[kMostSize / 2];
 };
 
@@ -172,131 +180,145 @@ __device__ inline void make_table(const Args<T> &a, uint32_t n0, uint32_t count,
 }
 
 // BACK: gradients.  NORM: with the norm of each head.
+//
+// Queries and keys take workgroups of their own (one launch), so that a workgroup needs one set of weights and sums; the
+// second computation of a token's angles costs less than the registers of the other set (gradients with 16/4 heads of 64:
+// 143 registers per lane and 53 us with both in one workgroup, 4 x 16 Ki tokens).
 template <typename T, int V, bool INTER, bool NORM, bool BACK>
 __global__ __launch_bounds__(kBlock) void rotary_kernel(const Args<T> a) {
   __shared__ float2 table[kMostTokens * (kMostSize / 2)];
   __shared__ uint32_t valid[kMostTokens];
+  constexpr uint32_t U = V > 1 && !(NORM && BACK) ? 2 : 1;  // rows at a time, their loads in flight together
+  const Side<T> &side = a.side[blockIdx.y];
+  if (blockIdx.x >= side.blocks) return;
   const uint32_t l = threadIdx.x & (a.lanes - 1), group = threadIdx.x / a.lanes, groups = kBlock / a.lanes;
   const Place<V, INTER> at(l, a.pairs, a.items, a.d);
   const float inv_d = 1.f / (float)a.d;
 
-  float wq[NORM ? 2 * V : 1], wk[NORM ? 2 * V : 1], sq[NORM && BACK ? 2 * V : 1], sk[NORM && BACK ? 2 * V : 1];
+  float w[NORM ? 2 * V : 1], sums_of[NORM && BACK ? 2 * V : 1];
   if constexpr (NORM) {
-    load_row<T, V>(a.wq, at.a, at.b, at.use, at.use_b, wq);
-    if (a.h > a.hq) load_row<T, V>(a.wk, at.a, at.b, at.use, at.use_b, wk);
+    load_row<T, V>(side.w, at.a, at.b, at.use, at.use_b, w);
     if constexpr (BACK) {
 #pragma unroll
-      for (int i = 0; i < 2 * V; ++i) sq[i] = sk[i] = 0.f;
+      for (int i = 0; i < 2 * V; ++i) sums_of[i] = 0.f;
     }
   }
 
-  for (uint64_t n = (uint64_t)blockIdx.x * a.tt; n < a.tokens; n += (uint64_t)gridDim.x * a.tt) {
-    const uint32_t n0 = (uint32_t)n, count = min(a.tt, a.tokens - n0), rows = count * a.h;
+  for (uint64_t n = (uint64_t)blockIdx.x * side.tt; n < a.tokens; n += (uint64_t)side.blocks * side.tt) {
+    const uint32_t n0 = (uint32_t)n, count = min(side.tt, a.tokens - n0), rows = count * side.heads;
+    const size_t base = (size_t)n0 * side.heads * a.d;
     make_table(a, n0, count, table, valid);
     __syncthreads();
-    for (uint32_t r0 = 0; r0 < rows; r0 += groups) {
-      const bool exists = r0 + group < rows;
-      const uint32_t r = exists ? r0 + group : rows - 1;  // lanes without a row go along for the exchanges
-      const uint32_t t = r / a.h, head = r - t * a.h;
-      const bool is_q = head < a.hq;
-      const size_t off = is_q ? ((size_t)(n0 + t) * a.hq + head) * a.d : ((size_t)(n0 + t) * (a.h - a.hq) + (head - a.hq)) * a.d;
-      const bool in = valid[t] != 0;
-      const float2 *cs = table + t * (kMostSize / 2) + at.angle;
-      float z[2 * V];
-      T *out = (is_q ? a.oq : a.ok) + off;
-      if constexpr (!BACK) {
-        load_row<T, V>((is_q ? a.xq : a.xk) + off, at.a, at.b, at.use, at.use_b, z);
-        if constexpr (NORM) {
-          float ss = 0.f;
+    for (uint32_t r0 = 0; r0 < rows; r0 += groups * U) {
+      float z[U][2 * V];
+      bool exists[U], in[U];
+      size_t off[U];
+      const float2 *cs[U];
 #pragma unroll
-          for (int i = 0; i < 2 * V; ++i) ss = fmaf(z[i], z[i], ss);
-          const float inv = 1.f / sqrtf(fmaf(row_sum(ss, a.lanes), inv_d, a.eps));
+      for (uint32_t u = 0; u < U; ++u) {
+        const uint32_t ru = r0 + u * groups + group;
+        exists[u] = ru < rows;
+        const uint32_t r = exists[u] ? ru : rows - 1;  // lanes without a row go along for the exchanges
+        const uint32_t t = side.inv == 0 ? r : __umulhi(r, side.inv);
+        in[u] = valid[t] != 0;
+        cs[u] = table + t * (kMostSize / 2) + at.angle;
+        off[u] = base + (size_t)r * a.d;
+        if constexpr (!BACK) load_row<T, V>(side.x + off[u], at.a, at.b, at.use, at.use_b, z[u]);
+        else load_row<T, V>(side.gy + off[u], at.a, at.b, at.use && in[u], at.use_b && in[u], z[u]);
+      }
 #pragma unroll
-          for (int i = 0; i < 2 * V; ++i) z[i] = z[i] * inv * (is_q ? wq[i] : wk[i]);
-        }
-        if (at.turns) rotate<V, INTER>(z, cs, 1.f);
-        if (!in) {
+      for (uint32_t u = 0; u < U; ++u) {
+        T *out = side.o + off[u];
+        if constexpr (!BACK) {
+          if constexpr (NORM) {
+            float ss = 0.f;
 #pragma unroll
-          for (int i = 0; i < 2 * V; ++i) z[i] = 0.f;
-        }
-        if (exists) store_row<T, V>(out, at.a, at.b, at.use, at.use_b, false, z);
-      } else {
-        load_row<T, V>((is_q ? a.gyq : a.gyk) + off, at.a, at.b, at.use && in, at.use_b && in, z);
-        if (at.turns) rotate<V, INTER>(z, cs, -1.f);
-        if constexpr (NORM) {
-          float x[2 * V];
-          load_row<T, V>((is_q ? a.xq : a.xk) + off, at.a, at.b, at.use && in, at.use_b && in, x);
-          float ss = 0.f, dot = 0.f;
+            for (int i = 0; i < 2 * V; ++i) ss = fmaf(z[u][i], z[u][i], ss);
+            const float inv = 1.f / sqrtf(fmaf(row_sum(ss, a.lanes), inv_d, a.eps));
 #pragma unroll
-          for (int i = 0; i < 2 * V; ++i) {
-            ss = fmaf(x[i], x[i], ss);
-            dot = fmaf(z[i] * (is_q ? wq[i] : wk[i]), x[i], dot);
+            for (int i = 0; i < 2 * V; ++i) z[u][i] = z[u][i] * inv * w[i];
           }
-          const float inv = 1.f / sqrtf(fmaf(row_sum(ss, a.lanes), inv_d, a.eps));
-          const float mean = row_sum(dot, a.lanes) * inv_d * inv * inv;
+          if (at.turns) rotate<V, INTER>(z[u], cs[u], 1.f);
+          if (!in[u]) {
 #pragma unroll
-          for (int i = 0; i < 2 * V; ++i) {
-            const float g = z[i], add = exists ? g * x[i] * inv : 0.f;
-            sq[i] += is_q ? add : 0.f;
-            sk[i] += is_q ? 0.f : add;
-            z[i] = inv * (g * (is_q ? wq[i] : wk[i]) - x[i] * mean);
+            for (int i = 0; i < 2 * V; ++i) z[u][i] = 0.f;
           }
+          if (exists[u]) store_row<T, V>(out, at.a, at.b, at.use, at.use_b, false, z[u]);
+        } else {
+          if (at.turns) rotate<V, INTER>(z[u], cs[u], -1.f);
+          if constexpr (NORM) {
+            float x[2 * V];
+            load_row<T, V>(side.x + off[u], at.a, at.b, at.use && in[u], at.use_b && in[u], x);
+            float ss = 0.f, dot = 0.f;
+#pragma unroll
+            for (int i = 0; i < 2 * V; ++i) {
+              ss = fmaf(x[i], x[i], ss);
+              dot = fmaf(z[u][i] * w[i], x[i], dot);
+            }
+            const float inv = 1.f / sqrtf(fmaf(row_sum(ss, a.lanes), inv_d, a.eps));
+            const float mean = row_sum(dot, a.lanes) * inv_d * inv * inv;
+#pragma unroll
+            for (int i = 0; i < 2 * V; ++i) {
+              const float g = z[u][i];
+              sums_of[i] += exists[u] ? g * x[i] * inv : 0.f;
+              z[u][i] = inv * (g * w[i] - x[i] * mean);
+            }
+          }
+          const bool acc = side.acc != 0;
+          if (exists[u] && (in[u] || !acc)) store_row<T, V>(out, at.a, at.b, at.use, at.use_b, acc, z[u]);
         }
-        const bool acc = (is_q ? a.acc_q : a.acc_k) != 0;
-        if (exists && (in || !acc)) store_row<T, V>(out, at.a, at.b, at.use, at.use_b, acc, z);
       }
     }
     __syncthreads();
   }
 
   if constexpr (NORM && BACK) {
-    // the workgroup's sums: row groups one after another, in a fixed order
-    __shared__ float sums[2 * kMostSize];
-    for (uint32_t i = threadIdx.x; i < 2 * kMostSize; i += kBlock) sums[i] = 0.f;
-    // first between the rows of a wavefront
+    // the workgroup's sums: first between the rows of a wavefront, then wavefront after wavefront, in a fixed order
+    __shared__ float sums[kMostSize];
+    for (uint32_t i = threadIdx.x; i < kMostSize; i += kBlock) sums[i] = 0.f;
 #pragma unroll
     for (int i = 0; i < 2 * V; ++i)
-      for (uint32_t o = a.lanes; o < 64; o <<= 1) {
-        sq[i] += __shfl_xor(sq[i], (int)o);
-        sk[i] += __shfl_xor(sk[i], (int)o);
-      }
-    for (uint32_t w = 0; w < kBlock / 64; ++w) {
+      for (uint32_t o = a.lanes; o < 64; o <<= 1) sums_of[i] += __shfl_xor(sums_of[i], (int)o);
+    for (uint32_t v = 0; v < kBlock / 64; ++v) {
       __syncthreads();
-      if (threadIdx.x / 64 == w && (threadIdx.x & 63) < a.lanes) {
+      if (threadIdx.x / 64 == v && (threadIdx.x & 63) < a.lanes) {
 #pragma unroll
         for (int i = 0; i < V; ++i) {
-          if (at.use) {
-            sums[at.a + i] += sq[i];
-            sums[kMostSize + at.a + i] += sk[i];
-          }
-          if (at.use_b) {
-            sums[at.b + i] += sq[V + i];
-            sums[kMostSize + at.b + i] += sk[V + i];
-          }
+          if (at.use) sums[at.a + i] += sums_of[i];
+          if (at.use_b) sums[at.b + i] += sums_of[V + i];
         }
       }
     }
     __syncthreads();
-    for (uint32_t i = threadIdx.x; i < 2 * a.d; i += kBlock)
-      a.partial[(size_t)blockIdx.x * 2 * a.d + i] = i < a.d ? sums[i] : sums[kMostSize + i - a.d];
+    for (uint32_t i = threadIdx.x; i < a.d; i += kBlock)
+      a.partial[((size_t)(blockIdx.y ? a.side[0].blocks : 0) + blockIdx.x) * a.d + i] = sums[i];
   }
 }
 
-// gw (+)= the sum over the workgroups of one column of the partial sums: a workgroup takes 16 columns, 16 threads each.
+// gw (+)= the sum over the workgroups of a side of one column of the partial sums: a workgroup takes 16 columns, 16 threads
+// each.
 template <typename T>
-__global__ __launch_bounds__(kBlock) void weights_kernel(const float *partial, uint32_t blocks, uint32_t d, T *gwq, T *gwk,
-                                                         uint32_t acc_q, uint32_t acc_k) {
+__global__ __launch_bounds__(kBlock) void weights_kernel(const float *partial, uint32_t blocks_q, uint32_t blocks_k, uint32_t d,
+                                                         T *gwq, T *gwk, uint32_t acc_q, uint32_t acc_k) {
   __shared__ float part[kBlock];
-  const uint32_t c = blockIdx.x * 16 + (threadIdx.x & 15), k = threadIdx.x >> 4;
+  const bool is_q = blockIdx.y == 0;
+  const uint32_t c = blockIdx.x * 16 + (threadIdx.x & 15), k = threadIdx.x >> 4, blocks = is_q ? blocks_q : blocks_k;
+  const float *from = partial + (is_q ? 0 : (size_t)blocks_q * d);
   float s = 0.f;
-  if (c < 2 * d)
-    for (uint32_t b = k; b < blocks; b += 16) s += partial[(size_t)b * 2 * d + c];
+  if (c < d)
+    for (uint32_t b0 = k; b0 < blocks; b0 += 16 * 16) {  // 16 loads in flight
+      float x[16];
+#pragma unroll
+      for (uint32_t u = 0; u < 16; ++u) x[u] = b0 + 16 * u < blocks ? from[(size_t)(b0 + 16 * u) * d + c] : 0.f;
+#pragma unroll
+      for (uint32_t u = 0; u < 16; ++u) s += x[u];
+    }
   part[threadIdx.x] = s;
   __syncthreads();
-  if (k != 0 || c >= 2 * d) return;
+  if (k != 0 || c >= d) return;
   for (uint32_t i = 1; i < 16; ++i) s += part[threadIdx.x + 16 * i];
-  T *p = c < d ? gwq + c : gwk != nullptr ? gwk + (c - d) : nullptr;
-  if (p != nullptr) *p = from_f32<T>((c < d ? acc_q : acc_k) ? to_f32(*p) + s : s);
+  T *p = (is_q ? gwq : gwk) + c;
+  *p = from_f32<T>((is_q ? acc_q : acc_k) ? to_f32(*p) + s : s);
 }
 
 // What the four entry points share.
@@ -306,7 +328,7 @@ int make_args(phip_ctx *ctx, uint32_t d, uint32_t hq, uint32_t hk, uint32_t t, u
   PHIP_REQUIRE(d >= 1 && d <= kMostSize, "head sizes of 1 to %u are supported, got %u", kMostSize, d);
   PHIP_REQUIRE(hq >= 1 && t >= 1 && bs >= 1, "empty tensors");
   PHIP_REQUIRE(has_k ? hk >= 1 : hk == 0, "%u heads of keys, and the keys are %s", hk, has_k ? "given" : "null");
-  PHIP_REQUIRE((uint64_t)hq + hk <= (1u << 20), "too many heads");
+  PHIP_REQUIRE(hq <= 16384 && hk <= 16384, "more than 16384 heads");  // rows of 8 tokens divided by a multiplication
   PHIP_REQUIRE(pairs <= d / 2, "%u pairs in a head of %u elements", pairs, d);
   PHIP_REQUIRE(pairs == 0 || freqs != nullptr, "null frequencies");
   PHIP_REQUIRE(eps >= 0.f && eps <= 3.4e38f, "eps must be finite and not negative");
@@ -316,8 +338,11 @@ int make_args(phip_ctx *ctx, uint32_t d, uint32_t hq, uint32_t hk, uint32_t t, u
   if (rc != PHIP_OK) return rc;
   a.tokens = t * bs;
   a.d = d;
-  a.hq = hq;
-  a.h = hq + hk;
+  for (int i = 0; i < 2; ++i) {
+    const uint32_t h = i == 0 ? hq : hk;
+    a.side[i].heads = h;
+    a.side[i].inv = h <= 1 ? 0 : (uint32_t)(((1ull << 32) + h - 1) / h);
+  }
   a.pairs = pairs;
   a.first = first;
   a.amplitude = amplitude;
@@ -330,41 +355,44 @@ int make_args(phip_ctx *ctx, uint32_t d, uint32_t hq, uint32_t hk, uint32_t t, u
 inline bool aligned(const void *p, size_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
 
 template <typename T, int V, bool INTER, bool NORM, bool BACK>
-int launch_kernel(phip_ctx *ctx, Args<T> a, uint32_t blocks) {
+int launch_kernel(phip_ctx *ctx, Args<T> a) {
   a.items = a.pairs / V + (a.d - 2 * a.pairs + 2 * V - 1) / (2 * V);
   a.lanes = 1;
   while (a.lanes < a.items) a.lanes *= 2;
-  hipLaunchKernelGGL((rotary_kernel<T, V, INTER, NORM, BACK>), dim3(blocks), dim3(kBlock), 0, ctx->stream, a);
+  const uint32_t blocks = std::max(a.side[0].blocks, a.side[1].blocks);
+  hipLaunchKernelGGL((rotary_kernel<T, V, INTER, NORM, BACK>), dim3(blocks, a.side[1].heads != 0 ? 2 : 1), dim3(kBlock), 0,
+                     ctx->stream, a);
   PHIP_LAUNCH_CHECK();
   return PHIP_OK;
 }
 
 template <typename T, bool NORM, bool BACK>
-int launch(phip_ctx *ctx, const Args<T> &a, bool interleaved, uint32_t blocks) {
+int launch(phip_ctx *ctx, const Args<T> &a, bool interleaved) {
   constexpr uint32_t W = 16 / sizeof(T);
   auto fits = [&](uint32_t v) {
     bool ok = a.d % v == 0 && a.pairs % v == 0;
-    for (const void *p : {(const void *)a.xq, (const void *)a.xk, (const void *)a.wq, (const void *)a.wk, (const void *)a.gyq,
-                          (const void *)a.gyk, (const void *)a.oq, (const void *)a.ok})
-      ok = ok && aligned(p, v * sizeof(T));
+    for (const Side<T> &s : a.side)
+      ok = ok && aligned(s.x, v * sizeof(T)) && aligned(s.w, v * sizeof(T)) && aligned(s.gy, v * sizeof(T)) && aligned(s.o, v * sizeof(T));
     return ok;
   };
-  if (fits(W))
-    return interleaved ? launch_kernel<T, W, true, NORM, BACK>(ctx, a, blocks) : launch_kernel<T, W, false, NORM, BACK>(ctx, a, blocks);
-  if (sizeof(T) == 2 && fits(2))
-    return interleaved ? launch_kernel<T, 2, true, NORM, BACK>(ctx, a, blocks) : launch_kernel<T, 2, false, NORM, BACK>(ctx, a, blocks);
-  return interleaved ? launch_kernel<T, 1, true, NORM, BACK>(ctx, a, blocks) : launch_kernel<T, 1, false, NORM, BACK>(ctx, a, blocks);
+  if (fits(W)) return interleaved ? launch_kernel<T, W, true, NORM, BACK>(ctx, a) : launch_kernel<T, W, false, NORM, BACK>(ctx, a);
+  if constexpr (sizeof(T) == 2) {
+    if (fits(2)) return interleaved ? launch_kernel<T, 2, true, NORM, BACK>(ctx, a) : launch_kernel<T, 2, false, NORM, BACK>(ctx, a);
+  }
+  return interleaved ? launch_kernel<T, 1, true, NORM, BACK>(ctx, a) : launch_kernel<T, 1, false, NORM, BACK>(ctx, a);
 }
 
-// Tokens per step: as many as leave a few workgroups for every CU.
+// Tokens per step of a side's workgroups: as many as leave a few workgroups for every CU.  looping: every workgroup leaves
+// a row of partial sums, so their number is limited and they take several steps.
 template <typename T>
-uint32_t choose(phip_ctx *ctx, Args<T> *a, bool looping) {
+void choose(phip_ctx *ctx, Args<T> *a, bool looping) {
   const uint64_t cus = (uint64_t)ctx->prop.multiProcessorCount;
-  uint64_t tt = a->tokens / (cus * 8);
-  a->tt = (uint32_t)(tt < 1 ? 1 : tt > kMostTokens ? kMostTokens : tt);
-  uint64_t blocks = (a->tokens + a->tt - 1) / a->tt;
-  const uint64_t cap = looping ? cus * 4 : ~0ull;  // looping: every workgroup leaves a row of partial sums
-  return (uint32_t)(blocks > cap ? cap : blocks);
+  for (Side<T> &s : a->side) {
+    if (s.heads == 0) continue;
+    const uint64_t tt = a->tokens / (cus * 8), blocks_cap = looping ? cus * 4 : ~0ull;
+    s.tt = (uint32_t)(tt < 1 ? 1 : tt > kMostTokens ? kMostTokens : tt);
+    s.blocks = (uint32_t)std::min<uint64_t>((a->tokens + s.tt - 1) / s.tt, blocks_cap);
+  }
 }
 
 template <typename T, bool NORM>
@@ -385,28 +413,28 @@ int forward(phip_ctx *ctx, const T *xq, const T *xk, const T *wq, const T *wk, T
   // a result may take its own operand's place; nothing else may overlap
   PHIP_REQUIRE(!read(yq, nq) && yq != xk && (yk == nullptr || (!read(yk, nk) && yk != xq && !shares_memory(yq, nq, yk, nk))),
                "a result shares memory with an operand or with the other result");
-  a.xq = xq;
-  a.xk = xk;
-  a.wq = wq;
-  a.wk = wk;
-  a.oq = yq;
-  a.ok = yk;
-  const uint32_t blocks = choose(ctx, &a, false);
-  return launch<T, NORM, false>(ctx, a, interleaved != 0, blocks);
+  a.side[0].x = xq;
+  a.side[1].x = xk;
+  a.side[0].w = wq;
+  a.side[1].w = wk;
+  a.side[0].o = yq;
+  a.side[1].o = yk;
+  choose(ctx, &a, false);
+  return launch<T, NORM, false>(ctx, a, interleaved != 0);
 }
 
 template <typename T, bool NORM>
 int backward_one(phip_ctx *ctx, Args<T> a, bool interleaved, T *gwq, T *gwk, bool acc_wq, bool acc_wk) {
-  const uint32_t blocks = choose(ctx, &a, NORM);
-  if constexpr (!NORM) return launch<T, false, true>(ctx, a, interleaved, blocks);
+  choose(ctx, &a, NORM);
+  if constexpr (!NORM) return launch<T, false, true>(ctx, a, interleaved);
   void *partial = nullptr;
-  int rc = phip_pool_alloc(ctx, (size_t)blocks * 2 * a.d * sizeof(float), &partial, nullptr);
+  int rc = phip_pool_alloc(ctx, (size_t)(a.side[0].blocks + a.side[1].blocks) * a.d * sizeof(float), &partial, nullptr);
   if (rc != PHIP_OK) return rc;
   a.partial = static_cast<float *>(partial);
-  rc = launch<T, NORM, true>(ctx, a, interleaved, blocks);
+  rc = launch<T, NORM, true>(ctx, a, interleaved);
   if (rc == PHIP_OK) {
-    hipLaunchKernelGGL((weights_kernel<T>), dim3((2 * a.d + 15) / 16), dim3(kBlock), 0, ctx->stream, a.partial, blocks, a.d,
-                       gwq, gwk, acc_wq ? 1u : 0u, acc_wk ? 1u : 0u);
+    hipLaunchKernelGGL((weights_kernel<T>), dim3((a.d + 15) / 16, a.side[1].heads != 0 ? 2 : 1), dim3(kBlock), 0, ctx->stream,
+                       a.partial, a.side[0].blocks, a.side[1].blocks, a.d, gwq, gwk, acc_wq ? 1u : 0u, acc_wk ? 1u : 0u);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) rc = fail(PHIP_ERR_RUNTIME, "launching the sum of the weights' gradients failed: %s", hipGetErrorString(e));
   }
@@ -442,36 +470,27 @@ int backward(phip_ctx *ctx, const T *xq, const T *xk, const T *wq, const T *wk, 
                          (!has_k || gwq == gwk || !shares_memory(gwq, nw, gwk, nw))),
                "a gradient of the weights overlaps another gradient");
   // gradients noted as zero and not yet filled are written instead of added into
-  a.acc_q = !zeros_take(ctx, gxq, nq);
-  a.acc_k = has_k && !zeros_take(ctx, gxk, nk);
+  a.side[0].acc = !zeros_take(ctx, gxq, nq);
+  a.side[1].acc = has_k && !zeros_take(ctx, gxk, nk);
   const bool acc_wq = NORM && !zeros_take(ctx, gwq, nw), acc_wk = NORM && has_k && !zeros_take(ctx, gwk, nw);
   PHIP_FLUSH_ZEROS(ctx);
-  a.xq = xq;
-  a.xk = xk;
-  a.wq = wq;
-  a.wk = wk;
-  a.gyq = gyq;
-  a.gyk = gyk;
-  a.oq = gxq;
-  a.ok = gxk;
+  a.side[0].x = xq;
+  a.side[1].x = xk;
+  a.side[0].w = wq;
+  a.side[1].w = wk;
+  a.side[0].gy = gyq;
+  a.side[1].gy = gyk;
+  a.side[0].o = gxq;
+  a.side[1].o = gxk;
   if (!has_k || (gxq != gxk && (!NORM || gwq != gwk)))
     return backward_one<T, NORM>(ctx, a, interleaved != 0, gwq, gwk, acc_wq, acc_wk);
   // one tensor for both gradients (a tensor or a weight used as queries' and as keys'): one after the other
-  Args<T> q = a, k = a;
-  q.h = hq;
-  q.xk = q.wk = q.gyk = nullptr;
-  q.ok = nullptr;
-  rc = backward_one<T, NORM>(ctx, q, interleaved != 0, gwq, nullptr, acc_wq, false);
+  Args<T> one = a;
+  one.side[1] = Side<T>{};
+  rc = backward_one<T, NORM>(ctx, one, interleaved != 0, gwq, nullptr, acc_wq, false);
   if (rc != PHIP_OK) return rc;
-  k.h = k.hq = hk;
-  k.xq = xk;
-  k.wq = wk;
-  k.gyq = gyk;
-  k.oq = gxk;
-  k.acc_q = a.acc_k;
-  k.xk = k.wk = k.gyk = nullptr;
-  k.ok = nullptr;
-  return backward_one<T, NORM>(ctx, k, interleaved != 0, gwk, nullptr, acc_wk, false);
+  one.side[0] = a.side[1];
+  return backward_one<T, NORM>(ctx, one, interleaved != 0, gwk, nullptr, acc_wk, false);
 }
 
 }  // namespace
