@@ -57,7 +57,7 @@ constexpr int kKeys = sizeof(T) == 2 ? 64 : 32;
 
 // gq and delta: the loop of the forward kernel with P recomputed instead of the running softmax.
 template <typename T, int DP, bool DMA>
-__global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void queries_kernel(const BwArgs<T> a) {
+__global__ __launch_bounds__(kThreads, sizeof(T) == 2 && DMA ? 2 : 1) void queries_kernel(const BwArgs<T> a) {
   constexpr int KT = kKeys<T>, BM = 32 * kWaves;
   typedef Tile<T, DP> L;
   typedef TileLoader<T, DP, KT, kThreads, DMA> Loader;
@@ -102,8 +102,10 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void queries_kern
   }
   delta = halves_sum(delta);
   const float base = valid ? row_base(a.stats[row]) : INFINITY;
-  if (valid && lane < 32) a.values[row] = {base, delta};
 
+  // The sum of a row of dS is 0 but for the rounding of y in delta: what comes out instead is the correction of delta that
+  // the other kernel uses (gradients of keys in fp16: error 1.5 -> 1.4 times that of rounding the result alone).
+  float rest = 0.f;
   f32x16 acc[DP / 32];
 #pragma unroll
   for (int db = 0; db < DP / 32; ++db) acc[db] = f32x16{};
@@ -153,6 +155,7 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void queries_kern
       for (int i = 0; i < 16; ++i) {
         const float x = exp2_fast(fmaf(p[i], sh.scale_log2, -base)) * (dp[i] - delta);
         p[i] = masked && first + block_row(i) >= lim ? 0.f : x;
+        rest += p[i];
       }
       __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
@@ -163,6 +166,8 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void queries_kern
       }
     }
   }
+  rest = halves_sum(rest);
+  if (valid && lane < 32) a.values[row] = {base, delta + rest};
   if (exists) emit_row<T, DP>(a.gq + row * sh.d, acc, sh.scale, valid, a.acc_q, sh.d, a.vec != 0, lane);
 }
 
@@ -436,10 +441,10 @@ __global__ __launch_bounds__(64 * W, 1) void few_queries_kernel(const BwArgs<T> 
 
   delta = halves_sum(delta);
   const float base = valid ? row_base(a.stats[row]) : INFINITY;
-  if (valid && tid < 32) a.values[row] = {base, delta};
 
   arrived(qf);
   arrived(gf);
+  float rest = 0.f;  // corrects delta, as in queries_kernel
   f32x16 acc[DP / 32];
 #pragma unroll
   for (int db = 0; db < DP / 32; ++db) acc[db] = f32x16{};
@@ -467,6 +472,7 @@ __global__ __launch_bounds__(64 * W, 1) void few_queries_kernel(const BwArgs<T> 
     for (int i = 0; i < 16; ++i) {
       const float x = exp2_fast(fmaf(p[i], sh.scale_log2, -base)) * (dp[i] - delta);
       p[i] = masked && first + block_row(i) >= lim ? 0.f : x;
+      rest += p[i];
     }
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
@@ -480,6 +486,16 @@ __global__ __launch_bounds__(64 * W, 1) void few_queries_kernel(const BwArgs<T> 
     }
   }
   wait_loads<0>();
+  rest = halves_sum(rest);
+  if constexpr (W > 1) {
+    __shared__ float rests[W][32];
+    if (lane < 32) rests[wave][lane] = rest;
+    __syncthreads();
+    rest = 0.f;
+#pragma unroll
+    for (int w = 0; w < W; ++w) rest += rests[w][lane & 31];
+  }
+  if (valid && tid < 32) a.values[row] = {base, delta + rest};
   emit_sum<T, DP, W>(acc, lds, sh.scale, a.acc_q, sh.d, a.vec != 0,
                      [&](int i) { return i < exist ? a.gq + (row_0 + walk.at((uint32_t)i, sh.hq)) * sh.d : (T *)nullptr; },
                      filled);

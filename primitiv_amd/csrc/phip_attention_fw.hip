@@ -90,6 +90,70 @@ __device__ inline void softmax(Rows<DP> &st, Scores<KB> &sc, int key0, int lim, 
   st.l += sum;
 }
 
+// A value of a masked key may be infinite or no number: 0 times it must not reach the rows that do not see the key.  Tells
+// whether any of the fragment's elements is one.
+template <typename T>
+__device__ inline bool not_finite(const Frag16<T> &f) {
+  constexpr uint32_t kOnes = __is_same(T, bf16_t) ? 0x7f80u : 0x7c00u;
+  bool bad = false;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const uint32_t w = f.v[e];
+    bad = bad || (w & kOnes) == kOnes || ((w >> 16) & kOnes) == kOnes;
+  }
+  return bad;
+}
+__device__ inline bool not_finite(const f32x8 &f) {
+  bool bad = false;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) bad = bad || !(fabsf(f[j]) <= 3.4028234e38f);
+  return bad;
+}
+// The fragment with only element j of half h kept.
+template <typename T>
+__device__ inline Frag16<T> only(const Frag16<T> &f, int j, bool mine) {
+  Frag16<T> r;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) r.v[e] = mine && e == (j >> 1) ? f.v[e] & ((j & 1) ? 0xffff0000u : 0xffffu) : 0u;
+  return r;
+}
+__device__ inline f32x8 only(const f32x8 &f, int j, bool mine) {
+  f32x8 r;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) r[e] = mine && e == j ? f[e] : 0.f;
+  return r;
+}
+
+// The product with the values of a tile that holds masked keys.  If all values are finite it is the plain product; if not,
+// key after key is added to the rows that see it (slow, and rare: a value that is no number spoils the result anyway, only
+// not of the rows before it).
+template <typename T, int DP, int KB>
+__device__ inline bool values_masked(Rows<DP> &st, const Scores<KB> &sc, uint32_t v_at, int key0, int lim, int lane) {
+  bool bad = false;
+#pragma unroll
+  for (int rc = 0; rc < 2 * KB; ++rc)
+#pragma unroll
+    for (int db = 0; db < DP / 32; ++db) bad = bad || not_finite(Tile<T, DP>::col_frag(v_at, rc, db));
+  if (!__any(bad)) return false;
+#pragma unroll
+  for (int rc = 0; rc < 2 * KB; ++rc) {
+    const Frag<T> p = as_operand(sc.s[rc / 2], rc % 2, (Frag<T> *)nullptr);
+#pragma unroll
+    for (int db = 0; db < DP / 32; ++db) {
+      const Frag<T> v = Tile<T, DP>::col_frag(v_at, rc, db);
+#pragma unroll 1
+      for (int k = 0; k < 16; ++k) {
+        const int h = k >> 3, j = k & 7, key = key0 + 16 * rc + (j & 3) + 8 * (j >> 2) + 4 * h;
+        f32x16 one = f32x16{};
+        mma(one, only(v, j, (lane >> 5) == h), only(p, j, (lane >> 5) == h));
+#pragma unroll
+        for (int i = 0; i < 16; ++i) st.o[db][i] += key < lim ? one[i] : 0.f;
+      }
+    }
+  }
+  return true;
+}
+
 // The product with the values.
 template <typename T, int DP, int KB>
 __device__ inline void values(Rows<DP> &st, const Scores<KB> &sc, uint32_t v_at) {
@@ -203,7 +267,9 @@ __global__ __launch_bounds__(kThreads, 2) void rows_kernel(const FwArgs<T> a) {
       Scores<KT / 32> sc;
       scores<T, DP, KT / 32>(sc, qf, stage + row_at);
       softmax<DP, KT / 32>(st, sc, t * KT, lim, (t + 1) * KT > w_all, sh.scale_log2, lane);
-      values<T, DP, KT / 32>(st, sc, stage + kTile + col_at);
+      const bool masked = (t + 1) * KT > w_all;
+      if (!masked || !values_masked<T, DP, KT / 32>(st, sc, stage + kTile + col_at, t * KT, lim, lane))
+        values<T, DP, KT / 32>(st, sc, stage + kTile + col_at);
     }
   }
 
@@ -275,7 +341,8 @@ __global__ __launch_bounds__(64 * W, 1) void few_kernel(const FwArgs<T> a) {
   auto seen_by = [&](int rr) { return sh.causal ? min(lk, max(0, rr / g + lk - lq + 1)) : lk; };
   const bool exists = (lane & 31) < rows, valid = (lane & 31) < filled;
   const int lim = valid ? seen_by(r0 + (lane & 31)) : 0;
-  const int keys = filled <= 0 ? 0 : seen_by(r0 + filled - 1), all = filled < BM ? 0 : seen_by(r0);
+  const int keys = filled <= 0 ? 0 : seen_by(r0 + filled - 1), first_sees = filled <= 0 ? 0 : seen_by(r0);
+  const int all = filled < BM ? 0 : first_sees;
   const uint32_t ranges = max(1u, ((uint32_t)keys + a.chunk - 1) / a.chunk);
   if (range >= ranges) return;
   const int from = (int)(range * a.chunk), to = min(keys, from + (int)a.chunk);
@@ -324,7 +391,8 @@ __global__ __launch_bounds__(64 * W, 1) void few_kernel(const FwArgs<T> a) {
       fetch_k(key + S * kStep, s);
       softmax<DP, 1>(st, sc, key, lim, key + 32 > all, sh.scale_log2, lane);
       wait_loads<kInFlight>();
-      values<T, DP, 1>(st, sc, stage + kTile + col_at);
+      if (key + 32 <= first_sees || !values_masked<T, DP, 1>(st, sc, stage + kTile + col_at, key, lim, lane))
+        values<T, DP, 1>(st, sc, stage + kTile + col_at);
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
       fetch_v(key + S * kStep, s);
     }
@@ -344,7 +412,8 @@ __global__ __launch_bounds__(64 * W, 1) void few_kernel(const FwArgs<T> a) {
       Scores<1> sc;
       scores<T, DP, 1>(sc, qf, ring + row_at);
       softmax<DP, 1>(st, sc, key, lim, key + 32 > all, sh.scale_log2, lane);
-      values<T, DP, 1>(st, sc, ring + kTile + col_at);
+      if (key + 32 <= first_sees || !values_masked<T, DP, 1>(st, sc, ring + kTile + col_at, key, lim, lane))
+        values<T, DP, 1>(st, sc, ring + kTile + col_at);
     }
   }
 
