@@ -525,7 +525,17 @@ template <typename T, int DP>
 constexpr int kStages = 32 * Tile<T, DP>::kPitch <= 8192 ? 2 : 1;
 
 // Which kernel walks over a call's tiles: the one whose workgroup shares every tile between 128 rows (or keys), or the one
-// where each wavefront walks over tiles of its own, 4 or 1 of them with the same 32 rows (keys).
+// where each wavefront walks over tiles of its own, four or one of them with the same 32 rows (keys).
+//
+// Shared tiles cost the least per product, so they are taken wherever their workgroups fill the chip; with one for every
+// second CU or fewer the finer division wins.  Both sides, us per training step, causal:
+//   bf16, 16/4 heads of 128:   4 x 128 tokens 70 -> 41,   4 x 512 192 -> 94,   1 x 2048 672 -> 281
+//   fp32, 16/4 heads of 128:   4 x 128       223 -> 83,   4 x 512 803 -> 360,  1 x 2048 3129 -> 1085
+//   and the other way with a workgroup per CU: bf16, 16 heads of 65, 4 x 512: 149 shared, 301 with tiles of their own.
+// fp32 products take four times as long per tile, which hides the loads of the finer division: there it also wins with a
+// workgroup per CU when the walk is long (16 heads of 65, 1 x 2048: 1068 -> 740).
+// One wavefront per workgroup: fp32 sequences so short that a 128-row tile is mostly empty and so many that every SIMD has
+// one anyway (16 heads of 65, 64 x 35 tokens: 217 -> 157; in 16-bit storage it does not pay: 125 against 157).
 enum class Way { Shared, Four, One };
 // wide, narrow: workgroups with tiles of 128 and of 32; most: rows (keys) of the longest sequence; walked: what its
 // workgroups walk over.

@@ -8,6 +8,7 @@
 // gq in memory, the same bits on every run.  The heads that share a key head are rows of one problem (as in the forward
 // kernel), so their contributions to gk and gv meet in the same registers.
 #include <algorithm>
+#include <type_traits>
 
 #include "phip_attention.h"
 
@@ -56,8 +57,13 @@ template <typename T>
 constexpr int kKeys = sizeof(T) == 2 ? 64 : 32;
 
 // gq and delta: the loop of the forward kernel with P recomputed instead of the running softmax.
-template <typename T, int DP, bool DMA>
-__global__ __launch_bounds__(kThreads, sizeof(T) == 2 && DMA ? 2 : 1) void queries_kernel(const BwArgs<T> a) {
+//
+// delta comes from y as it was stored.  In 16-bit storage its rounding is an error e of delta that adds -e P k to gq, and with
+// few keys per row that shows (sequences of 6 to 19 tokens in bf16: gq 1.65 times as far off as its own rounding).  FIX adds
+// up P k as well, one more product on the fragments at hand, and takes e, which is minus the sum of a row of dS, back out:
+// for 16-bit storage and fewer than 1024 keys; behind that the error is lost among those of more terms (8192 keys: 1.4 times).
+template <typename T, int DP, bool DMA, bool FIX>
+__global__ __launch_bounds__(kThreads, sizeof(T) == 2 && DMA && !(FIX && DP == 128) ? 2 : 1) void queries_kernel(const BwArgs<T> a) {
   constexpr int KT = kKeys<T>, BM = 32 * kWaves;
   typedef Tile<T, DP> L;
   typedef TileLoader<T, DP, KT, kThreads, DMA> Loader;
@@ -109,6 +115,9 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 && DMA ? 2 : 1) void queri
   f32x16 acc[DP / 32];
 #pragma unroll
   for (int db = 0; db < DP / 32; ++db) acc[db] = f32x16{};
+  [[maybe_unused]] f32x16 pk[DP / 32];
+#pragma unroll
+  for (int db = 0; db < DP / 32; ++db) pk[db] = f32x16{};
   const uint32_t stride = sh.hk * sh.d;
   const T *kp = a.k + ((sample * a.seq.tk + e.k_start) * sh.hk + head) * (size_t)sh.d;
   const T *vp = a.v + ((sample * a.seq.tk + e.k_start) * sh.hk + head) * (size_t)sh.d;
@@ -150,11 +159,14 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 && DMA ? 2 : 1) void queri
 #pragma unroll
       for (int c = 0; c < DP / 16; ++c) mma(dp, L::row_frag(stage + kTile + row_at, kb, c), gf[c]);
       __builtin_amdgcn_sched_barrier(0);
+      [[maybe_unused]] f32x16 pp;
       const int first = t * KT + 32 * kb + 4 * (lane >> 5);
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
-        const float x = exp2_fast(fmaf(p[i], sh.scale_log2, -base)) * (dp[i] - delta);
-        p[i] = masked && first + block_row(i) >= lim ? 0.f : x;
+        const float e = exp2_fast(fmaf(p[i], sh.scale_log2, -base)), x = e * (dp[i] - delta);
+        const bool hidden = masked && first + block_row(i) >= lim;
+        if constexpr (FIX) pp[i] = hidden ? 0.f : e;
+        p[i] = hidden ? 0.f : x;
         rest += p[i];
       }
       __builtin_amdgcn_sched_barrier(0);
@@ -162,12 +174,22 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 && DMA ? 2 : 1) void queri
       for (int c = 0; c < 2; ++c) {
         const Frag<T> ds = as_operand(p, c, (Frag<T> *)nullptr);
 #pragma unroll
-        for (int db = 0; db < DP / 32; ++db) mma(acc[db], L::col_frag(stage + col_at, 2 * kb + c, db), ds);
+        for (int db = 0; db < DP / 32; ++db) {
+          const Frag<T> kt = L::col_frag(stage + col_at, 2 * kb + c, db);
+          mma(acc[db], kt, ds);
+          if constexpr (FIX) mma(pk[db], kt, as_operand(pp, c, (Frag<T> *)nullptr));
+        }
       }
     }
   }
   rest = halves_sum(rest);
   if (valid && lane < 32) a.values[row] = {base, delta + rest};
+  if constexpr (FIX) {
+#pragma unroll
+    for (int db = 0; db < DP / 32; ++db)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) acc[db][i] = fmaf(-rest, pk[db][i], acc[db][i]);
+  }
   if (exists) emit_row<T, DP>(a.gq + row * sh.d, acc, sh.scale, valid, a.acc_q, sh.d, a.vec != 0, lane);
 }
 
@@ -378,7 +400,7 @@ __device__ inline void emit_sum(const f32x16 (&x)[DP / 32], unsigned char *lds, 
   }
 }
 
-template <typename T, int DP, bool DMA, int W>
+template <typename T, int DP, bool DMA, int W, bool FIX>
 __global__ __launch_bounds__(64 * W, 1) void few_queries_kernel(const BwArgs<T> a) {
   constexpr int BM = 32, S = DMA ? kStages<T, DP> : 1;
   typedef Tile<T, DP> L;
@@ -448,6 +470,9 @@ __global__ __launch_bounds__(64 * W, 1) void few_queries_kernel(const BwArgs<T> 
   f32x16 acc[DP / 32];
 #pragma unroll
   for (int db = 0; db < DP / 32; ++db) acc[db] = f32x16{};
+  [[maybe_unused]] f32x16 pk[DP / 32];
+#pragma unroll
+  for (int db = 0; db < DP / 32; ++db) pk[db] = f32x16{};
   for (int s = 0; key < keys; key += kStep, s = s + 1 == S ? 0 : s + 1) {
     const uint32_t stage = ring + (uint32_t)s * 2 * kTile;
     if constexpr (DMA) {
@@ -467,18 +492,25 @@ __global__ __launch_bounds__(64 * W, 1) void few_queries_kernel(const BwArgs<T> 
 #pragma unroll
     for (int c = 0; c < DP / 16; ++c) mma(dp, L::row_frag(stage + kTile + row_at, 0, c), gf[c]);
     const bool masked = key + 32 > all;
+    [[maybe_unused]] f32x16 pp;
     const int first = key + 4 * (lane >> 5);
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
-      const float x = exp2_fast(fmaf(p[i], sh.scale_log2, -base)) * (dp[i] - delta);
-      p[i] = masked && first + block_row(i) >= lim ? 0.f : x;
+      const float e = exp2_fast(fmaf(p[i], sh.scale_log2, -base)), x = e * (dp[i] - delta);
+      const bool hidden = masked && first + block_row(i) >= lim;
+      if constexpr (FIX) pp[i] = hidden ? 0.f : e;
+      p[i] = hidden ? 0.f : x;
       rest += p[i];
     }
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
       const Frag<T> ds = as_operand(p, c, (Frag<T> *)nullptr);
 #pragma unroll
-      for (int db = 0; db < DP / 32; ++db) mma(acc[db], L::col_frag(stage + col_at, c, db), ds);
+      for (int db = 0; db < DP / 32; ++db) {
+        const Frag<T> kt = L::col_frag(stage + col_at, c, db);
+        mma(acc[db], kt, ds);
+        if constexpr (FIX) mma(pk[db], kt, as_operand(pp, c, (Frag<T> *)nullptr));
+      }
     }
     if constexpr (DMA) {
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the tile's reads are done before its place is filled again
@@ -496,6 +528,12 @@ __global__ __launch_bounds__(64 * W, 1) void few_queries_kernel(const BwArgs<T> 
     for (int w = 0; w < W; ++w) rest += rests[w][lane & 31];
   }
   if (valid && tid < 32) a.values[row] = {base, delta + rest};
+  if constexpr (FIX) {
+#pragma unroll
+    for (int db = 0; db < DP / 32; ++db)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) acc[db][i] = fmaf(-rest, pk[db][i], acc[db][i]);
+  }
   emit_sum<T, DP, W>(acc, lds, sh.scale, a.acc_q, sh.d, a.vec != 0,
                      [&](int i) { return i < exist ? a.gq + (row_0 + walk.at((uint32_t)i, sh.hq)) * sh.d : (T *)nullptr; },
                      filled);
@@ -616,14 +654,25 @@ int launch(phip_ctx *ctx, BwArgs<T> a, const phip_sequences *seqs) {
   const Way way_q = choose_way<T>(ctx, wide_q, narrow_q, most_q, most_k), way_k = choose_way<T>(ctx, wide_k, narrow_k, most_k, most_q);
   const uint64_t rows = (uint64_t)a.seq.tq * a.s.g, keys = a.seq.tk;
   a.tiles = (uint32_t)(way_q == Way::Shared ? (rows + 127) / 128 : (rows + 31) / 32);
-  int rc = way_q == Way::Shared ? launch_kernel<queries_kernel<T, DP, DMA>>(ctx, a, wide_q, kThreads, lds_q)
-           : way_q == Way::Four ? launch_kernel<few_queries_kernel<T, DP, DMA, 4>>(ctx, a, narrow_q, 256, kFewLds<T, DP, 4>)
-                                : launch_kernel<few_queries_kernel<T, DP, DMA, 1>>(ctx, a, narrow_q, 64, kFewLds<T, DP, 1>);
+  auto queries = [&](auto fix) {
+    constexpr bool FIX = decltype(fix)::value;
+    if (way_q == Way::Four)
+      return launch_kernel<few_queries_kernel<T, DP, DMA, 4, FIX>>(ctx, a, narrow_q, 256, kFewLds<T, DP, 4>);
+    if constexpr (sizeof(T) == 4) {
+      if (way_q == Way::One) return launch_kernel<few_queries_kernel<T, DP, DMA, 1, FIX>>(ctx, a, narrow_q, 64, kFewLds<T, DP, 1>);
+    }
+    return launch_kernel<queries_kernel<T, DP, DMA, FIX>>(ctx, a, wide_q, kThreads, lds_q);
+  };
+  int rc = PHIP_OK;
+  if constexpr (sizeof(T) == 2) rc = most_k < 1024 ? queries(std::true_type()) : queries(std::false_type());
+  else rc = queries(std::false_type());
   if (rc != PHIP_OK) return rc;
   a.tiles = (uint32_t)(way_k == Way::Shared ? (keys + 127) / 128 : (keys + 31) / 32);
-  return way_k == Way::Shared ? launch_kernel<keys_kernel<T, DP, DMA>>(ctx, a, wide_k, kThreads, lds_k)
-         : way_k == Way::Four ? launch_kernel<few_keys_kernel<T, DP, DMA, 4>>(ctx, a, narrow_k, 256, kFewLds<T, DP, 4>)
-                              : launch_kernel<few_keys_kernel<T, DP, DMA, 1>>(ctx, a, narrow_k, 64, kFewLds<T, DP, 1>);
+  if (way_k == Way::Four) return launch_kernel<few_keys_kernel<T, DP, DMA, 4>>(ctx, a, narrow_k, 256, kFewLds<T, DP, 4>);
+  if constexpr (sizeof(T) == 4) {
+    if (way_k == Way::One) return launch_kernel<few_keys_kernel<T, DP, DMA, 1>>(ctx, a, narrow_k, 64, kFewLds<T, DP, 1>);
+  }
+  return launch_kernel<keys_kernel<T, DP, DMA>>(ctx, a, wide_k, kThreads, lds_k);
 }
 
 template <typename T, bool DMA>

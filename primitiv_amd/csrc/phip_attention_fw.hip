@@ -580,7 +580,9 @@ int launch(phip_ctx *ctx, const FwArgs<T> &a, const phip_sequences *seqs) {
   const uint64_t most = (uint64_t)(seqs != nullptr ? seqs->max_q : a.seq.tq) * a.s.g;
   Way way = choose_way<T>(ctx, wide, narrow, most, seqs != nullptr ? seqs->max_k : a.seq.tk);
   if (way == Way::Shared && most <= 32) way = Way::Four;
-  if (way == Way::One) return launch_few<T, DP, DMA, 1>(ctx, a, seqs);
+  if constexpr (sizeof(T) == 4) {
+    if (way == Way::One) return launch_few<T, DP, DMA, 1>(ctx, a, seqs);
+  }
   if (way == Way::Four) return launch_few<T, DP, DMA, 4>(ctx, a, seqs);
   return launch_rows<T, DP, DMA>(ctx, a);
 }

@@ -80,6 +80,14 @@ public:
   // Off: every fill is launched when it is asked for.
   void set_deferred_zero_fill(bool on);
 
+  // For the operators of phip.h that the Device interface has no virtual for
+  // (rotary positions, head norms, attention over sequences): the context, and
+  // the addresses of this device's tensors.  A mutable address is taken before
+  // the others of a call, because taking it may clone a shared block.
+  phip_ctx *context() { return ctx_; }
+  const void *address(const Tensor &x) { return get_handle(x); }
+  void *mutable_address(Tensor &x) { return get_mutable_handle(x); }
+
 private:
   // ---- implemented -------------------------------------------------------
   std::shared_ptr<void> new_handle(const Shape &shape, std::size_t *const allocated_size) override;
