@@ -731,7 +731,8 @@ int phip_norm_rotary_bw_bf16(phip_ctx *ctx, const void *xq, const void *xk, cons
  * consecutive query heads.  causal != 0: query i of lq sees the keys up to
  * i + lk - lq of lk (the queries are the sequence's last tokens).  A row that
  * sees no key gives 0, and so do tokens of no sequence; what k and v hold
- * outside the sequences is never used.  d <= 128, scale > 0.
+ * outside the sequences, or where the mask hides it, never reaches y (the
+ * gradients need finite q, k, v and gy inside the sequences).  d <= 128, scale > 0.
  * stats (may be NULL): float [hq, tq] x bs, the logarithm of the sum of
  * exponentials of each row, which the gradients need; -inf where no key is
  * seen.  Few queries against many keys (the single tokens of a serving loop)

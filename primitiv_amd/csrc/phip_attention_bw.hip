@@ -7,6 +7,9 @@
 // and in exchange every gradient is summed in registers in a fixed order and written once: no atomics, no fp32 copy of
 // gq in memory, the same bits on every run.  The heads that share a key head are rows of one problem (as in the forward
 // kernel), so their contributions to gk and gv meet in the same registers.
+//
+// Bound like the forward kernel by the matrix and the vector pipe in turn: 2 x 8192 tokens, 32/8 heads of 128, bf16, causal:
+// gq 1.65 ms (3 products, 1000 TFLOP/s), gk and gv 2.5 ms (4 products, 880 TFLOP/s).
 #include <algorithm>
 #include <type_traits>
 
@@ -249,7 +252,9 @@ __device__ inline void keys_block(f32x16 (&gk)[DP / 32], f32x16 (&gv)[DP / 32], 
 }
 
 // gk and gv: a workgroup takes 128 keys, 32 per wavefront, and walks over the rows (queries of the group) that see any of
-// them in tiles of QT.
+// them in tiles of QT.  16-bit heads of 128 take 255 registers, 128 of them the sums, and the order of keys_block (P, its
+// product, dP, its product, nothing moved across) is what fits: with two workgroups per CU 2.5 ms instead of 4.6 with one,
+// and a spilled fragment, read back in the loop, would wait for the tiles on their way (3.4 ms).
 template <typename T>
 constexpr int kRows = sizeof(T) == 2 ? 64 : 32;
 
