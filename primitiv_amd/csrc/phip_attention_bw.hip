@@ -643,7 +643,6 @@ template <auto *KERNEL, typename T>
 int launch_kernel(phip_ctx *ctx, const BwArgs<T> &a, uint64_t blocks, int threads, int lds) {
   const int rc = allow_lds<KERNEL>(ctx, lds);
   if (rc != PHIP_OK) return rc;
-  PHIP_REQUIRE(blocks < 0x7fffffffu, "too many rows");
   hipLaunchKernelGGL(KERNEL, dim3((uint32_t)blocks), dim3((uint32_t)threads), lds, ctx->stream, a);
   PHIP_LAUNCH_CHECK();
   return PHIP_OK;
@@ -716,15 +715,16 @@ int backward(phip_ctx *ctx, const T *q, const T *k, const T *v, const T *y, cons
                    ((const void *)gq == gk || !shares_memory(gq, nq, gk, nk)) &&
                    ((const void *)gq == gv || !shares_memory(gq, nq, gv, nk)),
                "two gradients overlap without being the same tensor");
-  // gradients noted as zero and not yet filled are written instead of added into; gq is written before gk and gk before
-  // gv, so of gradients that are one tensor the first takes the note
+  PHIP_REQUIRE(slots(a.seq, 32, a.s.g, false) * hk < 0x7fffffffu && slots(a.seq, 32, 1, true) * hk < 0x7fffffffu, "too many rows");
+  void *values = nullptr;
+  rc = phip_pool_alloc(ctx, 2 * ns, &values, nullptr);
+  if (rc != PHIP_OK) return rc;
+  // Nothing is refused from here on: gradients noted as zero and not yet filled are written instead of added into.  gq is
+  // written before gk and gk before gv, so of gradients that are one tensor the first takes the note.
   a.acc_q = !zeros_take(ctx, gq, nq);
   a.acc_k = !zeros_take(ctx, gk, nk);
   a.acc_v = !zeros_take(ctx, gv, nk);
   PHIP_FLUSH_ZEROS(ctx);
-  void *values = nullptr;
-  rc = phip_pool_alloc(ctx, 2 * ns, &values, nullptr);
-  if (rc != PHIP_OK) return rc;
   a.q = q;
   a.k = k;
   a.v = v;

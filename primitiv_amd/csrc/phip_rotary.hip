@@ -188,7 +188,8 @@ template <typename T, int V, bool INTER, bool NORM, bool BACK>
 __global__ __launch_bounds__(kBlock) void rotary_kernel(const Args<T> a) {
   __shared__ float2 table[kMostTokens * (kMostSize / 2)];
   __shared__ uint32_t valid[kMostTokens];
-  constexpr uint32_t U = V > 1 && !(NORM && BACK) ? 2 : 1;  // rows at a time, their loads in flight together
+  // rows at a time, their loads in flight together (single elements: four, or two with a second operand)
+  constexpr uint32_t U = V > 1 ? (NORM && BACK ? 1 : 2) : NORM && BACK ? 2 : 4;
   const Side<T> &side = a.side[blockIdx.y];
   if (blockIdx.x >= side.blocks) return;
   const uint32_t l = threadIdx.x & (a.lanes - 1), group = threadIdx.x / a.lanes, groups = kBlock / a.lanes;
@@ -211,6 +212,7 @@ __global__ __launch_bounds__(kBlock) void rotary_kernel(const Args<T> a) {
     __syncthreads();
     for (uint32_t r0 = 0; r0 < rows; r0 += groups * U) {
       float z[U][2 * V];
+      [[maybe_unused]] float xs[NORM && BACK ? U : 1][2 * V];
       bool exists[U], in[U];
       size_t off[U];
       const float2 *cs[U];
@@ -225,6 +227,7 @@ __global__ __launch_bounds__(kBlock) void rotary_kernel(const Args<T> a) {
         off[u] = base + (size_t)r * a.d;
         if constexpr (!BACK) load_row<T, V>(side.x + off[u], at.a, at.b, at.use, at.use_b, z[u]);
         else load_row<T, V>(side.gy + off[u], at.a, at.b, at.use && in[u], at.use_b && in[u], z[u]);
+        if constexpr (NORM && BACK) load_row<T, V>(side.x + off[u], at.a, at.b, at.use && in[u], at.use_b && in[u], xs[u]);
       }
 #pragma unroll
       for (uint32_t u = 0; u < U; ++u) {
@@ -247,8 +250,7 @@ __global__ __launch_bounds__(kBlock) void rotary_kernel(const Args<T> a) {
         } else {
           if (at.turns) rotate<V, INTER>(z[u], cs[u], -1.f);
           if constexpr (NORM) {
-            float x[2 * V];
-            load_row<T, V>(side.x + off[u], at.a, at.b, at.use && in[u], at.use_b && in[u], x);
+            float (&x)[2 * V] = xs[u];
             float ss = 0.f, dot = 0.f;
 #pragma unroll
             for (int i = 0; i < 2 * V; ++i) {
@@ -423,23 +425,16 @@ int forward(phip_ctx *ctx, const T *xq, const T *xk, const T *wq, const T *wk, T
   return launch<T, NORM, false>(ctx, a, interleaved != 0);
 }
 
+// partial: room for the sums of both sides' workgroups (norm only).
 template <typename T, bool NORM>
-int backward_one(phip_ctx *ctx, Args<T> a, bool interleaved, T *gwq, T *gwk, bool acc_wq, bool acc_wk) {
-  choose(ctx, &a, NORM);
-  if constexpr (!NORM) return launch<T, false, true>(ctx, a, interleaved);
-  void *partial = nullptr;
-  int rc = phip_pool_alloc(ctx, (size_t)(a.side[0].blocks + a.side[1].blocks) * a.d * sizeof(float), &partial, nullptr);
-  if (rc != PHIP_OK) return rc;
-  a.partial = static_cast<float *>(partial);
-  rc = launch<T, NORM, true>(ctx, a, interleaved);
-  if (rc == PHIP_OK) {
-    hipLaunchKernelGGL((weights_kernel<T>), dim3((a.d + 15) / 16, a.side[1].heads != 0 ? 2 : 1), dim3(kBlock), 0, ctx->stream,
-                       a.partial, a.side[0].blocks, a.side[1].blocks, a.d, gwq, gwk, acc_wq ? 1u : 0u, acc_wk ? 1u : 0u);
-    const hipError_t e = hipGetLastError();
-    if (e != hipSuccess) rc = fail(PHIP_ERR_RUNTIME, "launching the sum of the weights' gradients failed: %s", hipGetErrorString(e));
-  }
-  phip_pool_free(ctx, partial);
-  return rc;
+int backward_one(phip_ctx *ctx, Args<T> a, bool interleaved, float *partial, T *gwq, T *gwk, bool acc_wq, bool acc_wk) {
+  a.partial = partial;
+  const int rc = launch<T, NORM, true>(ctx, a, interleaved);
+  if (!NORM || rc != PHIP_OK) return rc;
+  hipLaunchKernelGGL((weights_kernel<T>), dim3((a.d + 15) / 16, a.side[1].heads != 0 ? 2 : 1), dim3(kBlock), 0, ctx->stream,
+                     a.partial, a.side[0].blocks, a.side[1].blocks, a.d, gwq, gwk, acc_wq ? 1u : 0u, acc_wk ? 1u : 0u);
+  PHIP_LAUNCH_CHECK();
+  return PHIP_OK;
 }
 
 template <typename T, bool NORM>
@@ -469,7 +464,13 @@ int backward(phip_ctx *ctx, const T *xq, const T *xk, const T *wq, const T *wk, 
                          !shares_memory(gwk, nw, gxq, nq) && !shares_memory(gwk, nw, gxk, nk) &&
                          (!has_k || gwq == gwk || !shares_memory(gwq, nw, gwk, nw))),
                "a gradient of the weights overlaps another gradient");
-  // gradients noted as zero and not yet filled are written instead of added into
+  choose(ctx, &a, NORM);
+  void *partial = nullptr;
+  if (NORM) {
+    rc = phip_pool_alloc(ctx, (size_t)(a.side[0].blocks + a.side[1].blocks) * d * sizeof(float), &partial, nullptr);
+    if (rc != PHIP_OK) return rc;
+  }
+  // nothing is refused from here on: gradients noted as zero and not yet filled are written instead of added into
   a.side[0].acc = !zeros_take(ctx, gxq, nq);
   a.side[1].acc = has_k && !zeros_take(ctx, gxk, nk);
   const bool acc_wq = NORM && !zeros_take(ctx, gwq, nw), acc_wk = NORM && has_k && !zeros_take(ctx, gwk, nw);
@@ -482,15 +483,19 @@ int backward(phip_ctx *ctx, const T *xq, const T *xk, const T *wq, const T *wk, 
   a.side[1].gy = gyk;
   a.side[0].o = gxq;
   a.side[1].o = gxk;
-  if (!has_k || (gxq != gxk && (!NORM || gwq != gwk)))
-    return backward_one<T, NORM>(ctx, a, interleaved != 0, gwq, gwk, acc_wq, acc_wk);
-  // one tensor for both gradients (a tensor or a weight used as queries' and as keys'): one after the other
-  Args<T> one = a;
-  one.side[1] = Side<T>{};
-  rc = backward_one<T, NORM>(ctx, one, interleaved != 0, gwq, nullptr, acc_wq, false);
-  if (rc != PHIP_OK) return rc;
-  one.side[0] = a.side[1];
-  return backward_one<T, NORM>(ctx, one, interleaved != 0, gwk, nullptr, acc_wk, false);
+  float *const sums = static_cast<float *>(partial);
+  if (!has_k || (gxq != gxk && (!NORM || gwq != gwk))) {
+    rc = backward_one<T, NORM>(ctx, a, interleaved != 0, sums, gwq, gwk, acc_wq, acc_wk);
+  } else {
+    // one tensor for both gradients (a tensor or a weight used as queries' and as keys'): one after the other
+    Args<T> one = a;
+    one.side[1] = Side<T>{};
+    rc = backward_one<T, NORM>(ctx, one, interleaved != 0, sums, gwq, nullptr, acc_wq, false);
+    one.side[0] = a.side[1];
+    if (rc == PHIP_OK) rc = backward_one<T, NORM>(ctx, one, interleaved != 0, sums, gwk, nullptr, acc_wk, false);
+  }
+  if (partial != nullptr) phip_pool_free(ctx, partial);
+  return rc;
 }
 
 }  // namespace

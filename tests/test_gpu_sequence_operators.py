@@ -314,6 +314,11 @@ def test_refusals(devices):
     rc = _lib.lib().phip_attention_bw_f32(*args, big.handle(), big.handle() + 4 * 64, big.handle() + 4 * 64 * 4 * 6 * 3,
                                           64, 4, 2, 6, 6, 2, None, 1, 0.1)
     assert rc == _lib.PHIP_ERR_INVALID_ARGUMENT
+    # a gradient that was to be zero is, after a refused call too
+    noted = g(k)
+    with pytest.raises(pa.Error):
+        dev.attention_bw(q, k, k, y, y, stats, True, 0.0, good, g(q), noted, noted)
+    assert (noted.to_vector() == 0).all()
     # nothing was enqueued by the refused calls: the device works on
     assert np.isfinite(dev.attention_fw(q, k, k).to_vector()).all()
 
