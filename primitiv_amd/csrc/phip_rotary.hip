@@ -257,7 +257,8 @@ __global__ __launch_bounds__(kBlock) void rotary_kernel(const Args<T> a) {
               ss = fmaf(x[i], x[i], ss);
               dot = fmaf(z[u][i] * w[i], x[i], dot);
             }
-            const float inv = 1.f / sqrtf(fmaf(row_sum(ss, a.lanes), inv_d, a.eps));
+            // tokens of no sequence come as zeros, which with eps == 0 have no finite norm: they add nothing
+            const float r = 1.f / sqrtf(fmaf(row_sum(ss, a.lanes), inv_d, a.eps)), inv = in[u] ? r : 0.f;
             const float mean = row_sum(dot, a.lanes) * inv_d * inv * inv;
 #pragma unroll
             for (int i = 0; i < 2 * V; ++i) {
