@@ -261,8 +261,8 @@ int phip_matmul_bw_bf16(phip_ctx *ctx, const void *a, const void *b, const void 
 
 /* Which kernels the matrix products went to.  No counterpart in the reference
  * (its devices hand every product to a vendor GEMM).  Copies the names of the
- * GEMM kernels launched by this context's matmul and convolution calls since
- * the previous call into buf (space-separated, in launch order per stream;
+ * GEMM kernels launched by this context's matmul and convolution calls, and of
+ * the kernels of its attention calls, since the previous call into buf (space-separated, in launch order per stream;
  * truncated to buf_size; buf may be NULL), forgets them, and switches the
  * note-taking on (on != 0) or off (the default).  For benchmarks and tests
  * that report or assert the kernel family a shape is served by; costs nothing

@@ -640,11 +640,12 @@ __global__ __launch_bounds__(64 * W, 1) void few_keys_kernel(const BwArgs<T> a) 
 }
 
 template <auto *KERNEL, typename T>
-int launch_kernel(phip_ctx *ctx, const BwArgs<T> &a, uint64_t blocks, int threads, int lds) {
+int launch_kernel(phip_ctx *ctx, const char *name, const BwArgs<T> &a, uint64_t blocks, int threads, int lds) {
   const int rc = allow_lds<KERNEL>(ctx, lds);
   if (rc != PHIP_OK) return rc;
   hipLaunchKernelGGL(KERNEL, dim3((uint32_t)blocks), dim3((uint32_t)threads), lds, ctx->stream, a);
   PHIP_LAUNCH_CHECK();
+  note_kernel(ctx, name);
   return PHIP_OK;
 }
 
@@ -661,22 +662,22 @@ int launch(phip_ctx *ctx, BwArgs<T> a, const phip_sequences *seqs) {
   auto queries = [&](auto fix) {
     constexpr bool FIX = decltype(fix)::value;
     if (way_q == Way::Four)
-      return launch_kernel<few_queries_kernel<T, DP, DMA, 4, FIX>>(ctx, a, narrow_q, 256, kFewLds<T, DP, 4>);
+      return launch_kernel<few_queries_kernel<T, DP, DMA, 4, FIX>>(ctx, FIX ? "attention_few_queries_fix" : "attention_few_queries", a, narrow_q, 256, kFewLds<T, DP, 4>);
     if constexpr (sizeof(T) == 4) {
-      if (way_q == Way::One) return launch_kernel<few_queries_kernel<T, DP, DMA, 1, FIX>>(ctx, a, narrow_q, 64, kFewLds<T, DP, 1>);
+      if (way_q == Way::One) return launch_kernel<few_queries_kernel<T, DP, DMA, 1, FIX>>(ctx, "attention_few1_queries", a, narrow_q, 64, kFewLds<T, DP, 1>);
     }
-    return launch_kernel<queries_kernel<T, DP, DMA, FIX>>(ctx, a, wide_q, kThreads, lds_q);
+    return launch_kernel<queries_kernel<T, DP, DMA, FIX>>(ctx, FIX ? "attention_queries_fix" : "attention_queries", a, wide_q, kThreads, lds_q);
   };
   int rc = PHIP_OK;
   if constexpr (sizeof(T) == 2) rc = most_k < 1024 ? queries(std::true_type()) : queries(std::false_type());
   else rc = queries(std::false_type());
   if (rc != PHIP_OK) return rc;
   a.tiles = (uint32_t)(way_k == Way::Shared ? (keys + 127) / 128 : (keys + 31) / 32);
-  if (way_k == Way::Four) return launch_kernel<few_keys_kernel<T, DP, DMA, 4>>(ctx, a, narrow_k, 256, kFewLds<T, DP, 4>);
+  if (way_k == Way::Four) return launch_kernel<few_keys_kernel<T, DP, DMA, 4>>(ctx, "attention_few_keys", a, narrow_k, 256, kFewLds<T, DP, 4>);
   if constexpr (sizeof(T) == 4) {
-    if (way_k == Way::One) return launch_kernel<few_keys_kernel<T, DP, DMA, 1>>(ctx, a, narrow_k, 64, kFewLds<T, DP, 1>);
+    if (way_k == Way::One) return launch_kernel<few_keys_kernel<T, DP, DMA, 1>>(ctx, "attention_few1_keys", a, narrow_k, 64, kFewLds<T, DP, 1>);
   }
-  return launch_kernel<keys_kernel<T, DP, DMA>>(ctx, a, wide_k, kThreads, lds_k);
+  return launch_kernel<keys_kernel<T, DP, DMA>>(ctx, "attention_keys", a, wide_k, kThreads, lds_k);
 }
 
 template <typename T, bool DMA>

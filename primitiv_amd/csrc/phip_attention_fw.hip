@@ -539,6 +539,7 @@ int launch_rows(phip_ctx *ctx, FwArgs<T> a) {
   if (rc != PHIP_OK) return rc;
   hipLaunchKernelGGL((rows_kernel<T, DP, DMA>), dim3((uint32_t)blocks), dim3(kThreads), lds, ctx->stream, a);
   PHIP_LAUNCH_CHECK();
+  note_kernel(ctx, "attention_rows");
   return PHIP_OK;
 }
 
@@ -576,6 +577,7 @@ int launch_few(phip_ctx *ctx, FwArgs<T> a, const phip_sequences *seqs) {
   const hipError_t e = hipGetLastError();
   if (partial != nullptr) phip_pool_free(ctx, partial);
   if (e != hipSuccess) return fail(PHIP_ERR_RUNTIME, "launching the attention kernel failed: %s", hipGetErrorString(e));
+  note_kernel(ctx, W == 1 ? "attention_few1" : a.splits > 1 ? "attention_few_split" : "attention_few");
   return PHIP_OK;
 }
 

@@ -95,7 +95,7 @@ struct phip_ctx {
   bool fixed_mode = false;
   // The second lane for matrix products; null in the side lane's own context.
   phip::Lanes *lanes = nullptr;
-  // Names of the matrix-product kernels launched on this context since the last phip_gemm_trace call,
+  // Names of the matrix-product and attention kernels launched on this context since the last phip_gemm_trace call,
   // kept only while tracing is switched on (benchmarks and tests ask which kernel a shape went to).
   bool trace_on = false;
   std::string trace;
@@ -213,7 +213,7 @@ int lanes_wait_host(phip_ctx *ctx);
 int lanes_order_main_after_side(phip_ctx *ctx);
 int lanes_place(phip_ctx *ctx, const MemRange *ranges, int n, bool may_overlap, phip_ctx **run_on);
 
-// Notes that a matrix product went to the kernel `name` (phip_gemm_trace).
+// Notes that a matrix product or an attention call went to the kernel `name` (phip_gemm_trace).
 inline void note_kernel(phip_ctx *ctx, const char *name) {
   if (!ctx->trace_on || ctx->trace.size() > 4000) return;
   if (!ctx->trace.empty()) ctx->trace += ' ';

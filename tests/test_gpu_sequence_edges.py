@@ -4,7 +4,7 @@ import numpy as np
 import pytest
 
 import primitiv_amd as pa
-from sequence_reference import HALF, Rotary, TINY, places
+from sequence_reference import Attention, HALF, Rotary, TINY, places
 from test_gpu_sequence_operators import KINDS, check, devices, draw, rounded, tensor  # noqa: F401
 
 pytestmark = pytest.mark.gpu
@@ -52,3 +52,136 @@ def test_norm_without_eps_beside_tokens_of_no_sequence(devices, kind, add, lens,
             r = r + start[key].reshape(r.shape)
             tol = tol + HALF[kind] * (np.abs(r) + tol) + TINY[kind]
         check("g" + key, got, r, tol)
+
+
+# Shapes of which every call fills the chip several times over with 128-row tiles, forward, over queries and over keys:
+# (size, query heads, key heads, tq, tk, batch, q_lens, k_lens, packed, causal)
+LARGE = {
+    "whole": (64, 16, 8, 150, 150, 20, None, None, False, True),
+    "not_causal": (128, 8, 8, 70, 200, 35, None, None, False, False),
+    "grouped": (128, 12, 4, 300, 300, 25, None, None, False, True),
+    "size_1": (1, 8, 4, 140, 140, 40, None, None, False, True),
+    "size_5": (5, 8, 8, 130, 70, 40, None, None, False, False),
+    "size_20": (20, 9, 3, 200, 200, 50, None, None, False, True),
+    "size_33": (33, 8, 8, 99, 99, 35, None, None, False, True),
+    "size_65": (65, 10, 10, 135, 135, 20, None, None, False, True),
+    "size_66": (66, 8, 4, 150, 170, 40, None, None, False, True),
+    "size_95": (95, 6, 6, 140, 140, 25, None, None, False, False),
+    "size_127": (127, 8, 8, 90, 90, 35, None, None, False, True),
+    "fewer_keys_than_queries": (64, 8, 8, 200, 80, 35, None, None, False, True),
+    "padded": (64, 16, 8, 160, 160, 20, (160, 0, 1, 129, 64) * 4, None, False, True),
+    "padded_odd_size": (33, 8, 8, 150, 170, 20, (150, 0, 1, 129, 64) * 4, (3, 170, 5, 64, 129) * 4, False, False),
+    "packed": (64, 16, 8, 4200, 4300, 1, (70, 1, 0, 350, 128, 700) * 3, (70, 2, 9, 350, 0, 700) * 3, True, True),
+    "packed_odd_size": (65, 12, 12, 3000, 3000, 1, (70, 1, 0, 350, 128, 400) * 3, None, True, True),
+    "group_of_40": (16, 160, 4, 40, 140, 35, None, None, False, True),
+    "many_keys": (64, 8, 8, 70, 1100, 35, None, None, False, True),
+    "many_keys_odd_size": (65, 4, 4, 70, 1030, 70, None, None, False, True),
+}
+
+
+def attention_against_reference(dev, kind, shape, seed, kernels):
+    """Forward and gradients of one shape; `kernels`: what each of the three must have gone to."""
+    d, hq, hk, tq, tk, bs, q_lens, k_lens, packed, causal = shape
+    rng = np.random.default_rng(seed)
+    q, k, v, gy = (draw(rng, kind, bs, t, h, d) for t, h in ((tq, hq), (tk, hk), (tk, hk), (tq, hq)))
+    seqs = places(bs, tq, tk, q_lens, k_lens, packed)
+    scale = 1.0 / float(np.sqrt(d))
+    want = Attention(q, k, v, seqs, causal, scale, kind, gy)
+    used_q, used_k = np.zeros(q.shape[:2], bool), np.zeros(k.shape[:2], bool)
+    for b, aq, n, ak, m in seqs:
+        used_q[b, aq:aq + n] = used_k[b, ak:ak + m] = True
+    q[~used_q], k[~used_k], v[~used_k], gy[~used_q] = np.nan, np.nan, np.inf, np.nan
+    tq_, tk_, tv_, tg_ = (tensor(dev, x) for x in (q, k, v, gy))
+    lists = None if q_lens is None else dev.new_sequences(q_lens, k_lens, packed)
+    start = {n: draw(rng, kind, *x.shape) for n, x in (("gq", q), ("gk", k), ("gv", v))}
+    g = {n: tensor(dev, x) for n, x in start.items()}
+    dev.gemm_trace(True)
+    y, stats = dev.attention_fw(tq_, tk_, tv_, causal, scale, lists, stats=True)
+    dev.attention_bw(tq_, tk_, tv_, y, tg_, stats, causal, scale, lists, g["gq"], g["gk"], g["gv"])
+    went = dev.gemm_trace(False)
+    assert [w.replace("_fix", "") for w in went] == list(kernels), went
+    check("y", y.to_vector(), want.y, want.tol_y)
+    got = stats.to_vector().reshape(want.stats.shape)
+    assert np.array_equal(np.isneginf(got), np.isneginf(want.stats))
+    some = ~np.isneginf(want.stats)
+    check("stats", got[some], want.stats[some], want.tol_stats[some])
+    for n in ("gq", "gk", "gv"):
+        r, t = getattr(want, n) + start[n], getattr(want, "tol_" + n)
+        check(n, g[n].to_vector(), r, t + HALF[kind] * (np.abs(r) + t) + TINY[kind])
+    zeroed = {n: dev.new_tensor_by_constant(t.shape(), 0) for n, t in (("gq", tq_), ("gk", tk_), ("gv", tv_))}
+    dev.attention_bw(tq_, tk_, tv_, y, tg_, stats, causal, scale, lists, zeroed["gq"], zeroed["gk"], zeroed["gv"])
+    for n in ("gq", "gk", "gv"):
+        check(n + " over zeros", zeroed[n].to_vector(), getattr(want, n), getattr(want, "tol_" + n))
+    return went
+
+
+@pytest.mark.parametrize("name", sorted(LARGE))
+@pytest.mark.parametrize("kind", KINDS)
+def test_attention_with_tiles_of_128_rows(devices, kind, name):  # noqa: F811
+    """The kernels whose workgroups share tiles, which prompts and training go to."""
+    attention_against_reference(devices[kind], kind, LARGE[name], 30 + len(name),
+                                ("attention_rows", "attention_queries", "attention_keys"))
+
+
+# Short sequences, so many that every SIMD has one: in fp32 a wavefront each
+SHORT = {
+    "whole": (64, 16, 16, 35, 35, 33, None, None, False, True),
+    "odd_size": (65, 10, 10, 35, 35, 64, None, None, False, True),
+    "size_1": (1, 16, 16, 50, 50, 33, None, None, False, False),
+    "size_33": (33, 16, 16, 64, 64, 17, None, None, False, True),
+    "grouped": (128, 32, 16, 20, 31, 40, None, None, False, True),
+    "padded": (96, 16, 16, 60, 64, 36, (60, 0, 1, 33) * 9, (60, 9, 3, 64) * 9, False, True),
+    "packed": (80, 40, 40, 400, 430, 1, (33, 1, 0, 60, 17) * 3, (35, 1, 9, 64, 0) * 3, True, True),
+}
+
+
+@pytest.mark.parametrize("name", sorted(SHORT))
+def test_attention_with_a_wavefront_per_tile(devices, name):  # noqa: F811
+    attention_against_reference(devices["f32"], "f32", SHORT[name], 60 + len(name),
+                                ("attention_few1", "attention_few1_queries", "attention_few1_keys"))
+
+
+@pytest.mark.parametrize("size", (64, 65))
+@pytest.mark.parametrize("kind", KINDS)
+def test_attention_with_tiles_of_128_rows_before_a_value_that_is_no_number(devices, kind, size):  # noqa: F811
+    dev = devices[kind]
+    rng = np.random.default_rng(7)
+    bs, n, h = 20, 150, 8
+    q, k, v = (draw(rng, kind, bs, n, h, size) for _ in range(3))
+    want = Attention(q, k, v, places(bs, n, n), True, 0.125, kind)
+    first = 100   # rows from here on see it; it lies in the middle of a tile of keys
+    v[:, first, :, 5] = np.nan
+    v[:, first + 3, :, 7] = np.inf
+    k[:, n - 1] = np.nan
+    dev.gemm_trace(True)
+    y = dev.attention_fw(tensor(dev, q), tensor(dev, k), tensor(dev, v), True, 0.125).to_vector().reshape(want.y.shape)
+    assert dev.gemm_trace(False) == ["attention_rows"]
+    check("y", y[:, :first], want.y[:, :first], want.tol_y[:, :first])
+    assert np.isnan(y[:, first:, :, 5]).all() and not np.isfinite(y[:, first + 3:, :, 7]).any()
+    others = [i for i in range(size) if i not in (5, 7)]
+    check("other columns", y[:, first:-1][..., others], want.y[:, first:-1][..., others], want.tol_y[:, first:-1][..., others])
+    assert np.isnan(y[:, -1]).all()
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_attention_of_one_tensor_with_tiles_of_128_rows(devices, kind):  # noqa: F811
+    """The same tensor as queries, keys and values, with its one gradient; the same bits on every run."""
+    dev = devices[kind]
+    rng = np.random.default_rng(8)
+    x, gy = draw(rng, kind, 35, 135, 8, 64), draw(rng, kind, 35, 135, 8, 64)
+    want = Attention(x, x, x, places(35, 135, 135), True, 0.125, kind, gy)
+    t, tg = tensor(dev, x), tensor(dev, gy)
+    seen = []
+    for _ in range(3):
+        dev.gemm_trace(True)
+        y, stats = dev.attention_fw(t, t, t, True, 0.125, None, stats=True)
+        g = dev.new_tensor_by_constant(t.shape(), 0)
+        dev.attention_bw(t, t, t, y, tg, stats, True, 0.125, None, g, g, g)
+        went = [w.replace("_fix", "") for w in dev.gemm_trace(False)]
+        assert went == ["attention_rows", "attention_queries", "attention_keys"]
+        seen.append((y.to_vector(), g.to_vector()))
+    for other in seen[1:]:
+        assert all(np.array_equal(a, b) for a, b in zip(seen[0], other))
+    total = want.gq + want.gk + want.gv
+    tol = want.tol_gq + want.tol_gk + want.tol_gv + HALF[kind] * (np.abs(want.gq) + np.abs(want.gq + want.gk) + np.abs(total)) * 1.05
+    check("g", seen[0][1], total, tol)
