@@ -34,7 +34,7 @@ struct FwArgs {
 template <int DP>
 struct Rows {
   f32x16 o[DP / 32];
-  float m, l;           // l: this half's keys only
+  float m, l;           // l: this half's keys only, raised like the result
 };
 
 // One step over 32 KB keys whose rows lie in LDS, in three parts.  The scores:
@@ -52,8 +52,9 @@ __device__ inline void scores(Scores<KB> &sc, const Frag<T> (&qf)[DP / 16], uint
   }
 }
 
-// The running softmax: the scores become exp(score - maximum).  lim: keys below it are visible to the lane's row.
-template <int DP, int KB>
+// The running softmax: the scores become exp(score - maximum), raised by kRaise.  lim: keys below it are visible to the
+// lane's row.
+template <typename T, int DP, int KB>
 __device__ inline void softmax(Rows<DP> &st, Scores<KB> &sc, int key0, int lim, bool masked, float scale_log2, int lane) {
   f32x16 (&s)[KB] = sc.s;
   if (masked) {
@@ -79,12 +80,13 @@ __device__ inline void softmax(Rows<DP> &st, Scores<KB> &sc, int key0, int lim, 
       for (int i = 0; i < 16; ++i) st.o[db][i] *= alpha;
     st.m = mx;
   }
+  const float raised = base - kRaise<T>;
   float sum = 0.f;
 #pragma unroll
   for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
-      s[kb][i] = exp2_fast(fmaf(s[kb][i], scale_log2, -base));
+      s[kb][i] = exp2_fast(fmaf(s[kb][i], scale_log2, -raised));
       sum += s[kb][i];
     }
   st.l += sum;
@@ -270,7 +272,7 @@ __global__ __launch_bounds__(kThreads, 2) void rows_kernel(const FwArgs<T> a) {
     if (t * KT < w_keys) {
       Scores<KT / 32> sc;
       scores<T, DP, KT / 32>(sc, qf, stage + row_at);
-      softmax<DP, KT / 32>(st, sc, t * KT, lim, (t + 1) * KT > w_all, sh.scale_log2, lane);
+      softmax<T, DP, KT / 32>(st, sc, t * KT, lim, (t + 1) * KT > w_all, sh.scale_log2, lane);
       const bool masked = (t + 1) * KT > w_all;
       if (!masked || !values_masked<T, DP, KT / 32>(st, sc, stage + kTile + col_at, t * KT, lim, lane))
         values<T, DP, KT / 32>(st, sc, stage + kTile + col_at);
@@ -280,7 +282,7 @@ __global__ __launch_bounds__(kThreads, 2) void rows_kernel(const FwArgs<T> a) {
   const float l = halves_sum(st.l);
   if (!exists) return;
   store_row<T, DP>(a.y + row * sh.d, st.o, 1.f / l, valid && l != 0.f, sh.d, a.vec_y != 0, lane);
-  if (a.stats != nullptr && lane < 32) a.stats[row] = !valid || l == 0.f ? -INFINITY : fmaf(st.m, sh.scale, logf(l));
+  if (a.stats != nullptr && lane < 32) a.stats[row] = !valid || l == 0.f ? -INFINITY : fmaf(st.m, sh.scale, logf(l * kLower<T>));
 }
 
 // Few rows (a new token per sequence against its cache, short prompts): what takes the time is reading the keys and values
@@ -394,7 +396,7 @@ __global__ __launch_bounds__(64 * W, 1) void few_kernel(const FwArgs<T> a) {
       scores<T, DP, 1>(sc, qf, stage + row_at);
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the block's reads are done before its place is filled again
       fetch_k(key + S * kStep, s);
-      softmax<DP, 1>(st, sc, key, lim, key + 32 > all, sh.scale_log2, lane);
+      softmax<T, DP, 1>(st, sc, key, lim, key + 32 > all, sh.scale_log2, lane);
       wait_loads<kInFlight>();
       if (key + 32 <= first_sees || !values_masked<T, DP, 1>(st, sc, stage + kTile + col_at, key, lim, lane))
         values<T, DP, 1>(st, sc, stage + kTile + col_at);
@@ -416,7 +418,7 @@ __global__ __launch_bounds__(64 * W, 1) void few_kernel(const FwArgs<T> a) {
       }
       Scores<1> sc;
       scores<T, DP, 1>(sc, qf, ring + row_at);
-      softmax<DP, 1>(st, sc, key, lim, key + 32 > all, sh.scale_log2, lane);
+      softmax<T, DP, 1>(st, sc, key, lim, key + 32 > all, sh.scale_log2, lane);
       if (key + 32 <= first_sees || !values_masked<T, DP, 1>(st, sc, ring + kTile + col_at, key, lim, lane))
         values<T, DP, 1>(st, sc, ring + kTile + col_at);
     }
@@ -427,7 +429,7 @@ __global__ __launch_bounds__(64 * W, 1) void few_kernel(const FwArgs<T> a) {
     if (!exists) return;
     const size_t row = row_base + walk.at(lane & 31, sh.hq);
     store_row<T, DP>(a.y + row * sh.d, st.o, 1.f / l, valid && l != 0.f, sh.d, a.vec_y != 0, lane);
-    if (a.stats != nullptr && lane < 32) a.stats[row] = !valid || l == 0.f ? -INFINITY : fmaf(st.m, sh.scale, logf(l));
+    if (a.stats != nullptr && lane < 32) a.stats[row] = !valid || l == 0.f ? -INFINITY : fmaf(st.m, sh.scale, logf(l * kLower<T>));
     return;
   }
   // the wavefronts' results: per wavefront DP columns of 33 floats (rows across), then 32 maxima and 32 sums
@@ -456,7 +458,7 @@ __global__ __launch_bounds__(64 * W, 1) void few_kernel(const FwArgs<T> a) {
     const float f = l == 0.f ? 0.f : 1.f / l;
     const float four[4] = {o[0] * f, o[1] * f, o[2] * f, o[3] * f};
     if (dd < sh.d) store4<T, false>(a.y + at_row * sh.d + dd, four, (int)(sh.d - dd), a.vec_y != 0);
-    if (dd == 0 && a.stats != nullptr) a.stats[at_row] = l == 0.f ? -INFINITY : fmaf(m, sh.scale, logf(l));
+    if (dd == 0 && a.stats != nullptr) a.stats[at_row] = l == 0.f ? -INFINITY : fmaf(m, sh.scale, logf(l * kLower<T>));
   };
   for (uint32_t i = tid; i < (uint32_t)rows * (DP / 4); i += kThreads) {
     const int row = (int)(i / (DP / 4));
@@ -524,7 +526,7 @@ __global__ __launch_bounds__(64 * W, 1) void few_kernel(const FwArgs<T> a) {
     if (dd >= sh.d) continue;
     const size_t at_row = row_base + walk.at((uint32_t)row, sh.hq);
     a.y[at_row * sh.d + dd] = from_f32<T>(l == 0.f ? 0.f : o / l);
-    if (dd == 0 && a.stats != nullptr) a.stats[at_row] = l == 0.f ? -INFINITY : fmaf(m, sh.scale, logf(l));
+    if (dd == 0 && a.stats != nullptr) a.stats[at_row] = l == 0.f ? -INFINITY : fmaf(m, sh.scale, logf(l * kLower<T>));
   }
 }
 

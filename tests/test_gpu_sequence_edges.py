@@ -185,3 +185,25 @@ def test_attention_of_one_tensor_with_tiles_of_128_rows(devices, kind):  # noqa:
     total = want.gq + want.gk + want.gv
     tol = want.tol_gq + want.tol_gk + want.tol_gv + HALF[kind] * (np.abs(want.gq) + np.abs(want.gq + want.gk) + np.abs(total)) * 1.05
     check("g", seen[0][1], total, tol)
+
+
+@pytest.mark.parametrize("name,shape", (("few", (4, 2, 4096, 1)), ("split", (1, 1, 8192, 1)), ("large", (130, 8, 1500, 18))))
+def test_fp16_many_small_probabilities_beside_a_large_one(devices, name, shape):  # noqa: F811
+    """One key takes nearly all of the weight, with a value of zero: the result is what thousands of keys with weights of
+    2^-26 each add up to.  Rounded once each (h of itself), and the result once."""
+    dev = devices["f16"]
+    n, heads, m, bs = shape
+    rng = np.random.default_rng(23)
+    q, k, v = np.zeros((bs, n, heads, 64)), np.zeros((bs, m, heads, 64)), 32 + 4 * rng.standard_normal((bs, m, heads, 64))
+    q[..., 0], k[:, 5, :, 0], v[:, 5] = 1.0, 18.0, 0.0
+    k[..., 1] = rng.standard_normal(k.shape[:-1])
+    q[..., 1] = 0.25
+    q, k, v = (rounded(x, "f16") for x in (q, k, v))
+    want = Attention(q, k, v, places(bs, n, m), False, 1.0, "f16")
+    dev.gemm_trace(True)
+    y, stats = dev.attention_fw(*(tensor(dev, x) for x in (q, k, v)), False, 1.0, None, stats=True)
+    went = dev.gemm_trace(False)
+    assert went == [{"few": "attention_few_split", "split": "attention_few_split", "large": "attention_rows"}[name]]
+    # two halves of a step; scores of 18 are off by 70 x 2^-24 x 18 at most
+    check("y", y.to_vector(), want.y, np.abs(want.y) * (2 * 2.0 ** -11 + 2.0 ** -13) + 2.0 ** -25)
+    check("stats", stats.to_vector(), want.stats.reshape(-1), want.tol_stats.reshape(-1))
