@@ -53,8 +53,75 @@ __device__ inline void emit_row(T *row, const f32x16 (&x)[DP / 32], float f, boo
     }
 }
 
-// exp(score - stats) as a power of two; a row without keys has stats = -inf and must give 0.
-__device__ inline float row_base(float stats) { return stats == -INFINITY ? INFINITY : stats * kLog2e; }
+// exp(score - stats) as a power of two, raised by kRaise; a row without keys has stats = -inf and must give 0.
+template <typename T>
+__device__ inline float row_base(float stats) { return stats == -INFINITY ? INFINITY : stats * kLog2e - kRaise<T>; }
+
+// dS in fp16.  It is a probability, of thousands of keys perhaps, times a difference of any size: 2^-40 and 2^20 are ordinary
+// values, and fp16 has neither.  So a wavefront scales its dS by a power of two before it is rounded, and its sums with it:
+// the first block puts the largest between 2^9 and 2^13, and a block that exceeds 2^15 scales everything down to that again.
+// What is below 2^-23 of the largest so far loses bits; nothing overflows.  Eight maxima and a multiplication per 16 values
+// (queries: part of the multiply-add), the rest is rare: a training step with heads of 64 takes 3 to 4 % longer than with dS
+// rounded as it is (16 heads, 8192 tokens: 815 against 784 us), with heads of 128 no longer.
+template <typename T>
+constexpr bool kRanged = __is_same(T, f16_t);
+struct Range {
+  float scale = 1.f;   // the same in all lanes
+  bool known = false;  // some dS was not 0 yet
+};
+
+// m: the largest |x| of the lane's 16 values.  Returns what x and the sums were multiplied by.
+template <int N>
+__device__ inline float fit(Range &range, f32x16 &x, f32x16 (&sums)[N], float m) {
+  if (range.known && !__any(m > 0x1p15f)) return 1.f;
+  if (!__any(m > 0.f)) return 1.f;
+  float by = 1.f;
+  // steps of 16, as many as the range of a float has: infinite values stay what they are
+#pragma unroll 1
+  for (int i = 0; i < 24 && !__any(m * by >= 0x1p9f); ++i) by *= 0x1p4f;
+#pragma unroll 1
+  for (int i = 0; i < 24 && __any(m * by > 0x1p13f); ++i) by *= 0x1p-4f;
+  range.known = true;
+  range.scale *= by;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) x[i] *= by;
+#pragma unroll
+  for (int db = 0; db < N; ++db)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) sums[db][i] *= by;
+  return by;
+}
+template <int N>
+__device__ inline void settle(f32x16 (&sums)[N], float f) {
+#pragma unroll
+  for (int db = 0; db < N; ++db)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) sums[db][i] *= f;
+}
+
+// A block of the kernels over the keys: p, the scores, becomes dS (of fp16 scaled by the range, and `rest` with it); pp (FIX)
+// the probabilities.  Keys from lim on are hidden (first: the lane's first key).
+template <typename T, bool FIX, int N>
+__device__ inline void differences(f32x16 &p, f32x16 &pp, const f32x16 &dp, f32x16 (&sums)[N], float &rest, Range &range,
+                                   float scale_log2, float base, float delta, bool masked, int first, int lim) {
+  const float scaled_delta = kRanged<T> ? delta * range.scale : delta;
+  float m = 0.f;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    const float e = exp2_fast(fmaf(p[i], scale_log2, -base));
+    const float x = e * (kRanged<T> ? fmaf(dp[i], range.scale, -scaled_delta) : dp[i] - delta);
+    const bool hidden = masked && first + block_row(i) >= lim;
+    if constexpr (FIX) pp[i] = hidden ? 0.f : e;
+    p[i] = hidden ? 0.f : x;
+    if constexpr (kRanged<T>) m = fmaxf(m, fabsf(p[i]));
+    else rest += p[i];
+  }
+  if constexpr (kRanged<T>) {
+    rest *= fit(range, p, sums, m);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) rest += p[i];
+  }
+}
 
 template <typename T>
 constexpr int kKeys = sizeof(T) == 2 ? 64 : 32;
@@ -110,11 +177,12 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 && DMA && !(FIX && DP == 1
       for (int j = 0; j < 8; ++j) delta = fmaf(element(gf[c], j), element(yf[c], j), delta);
   }
   delta = halves_sum(delta);
-  const float base = valid ? row_base(a.stats[row]) : INFINITY;
+  const float base = valid ? row_base<T>(a.stats[row]) : INFINITY;
 
   // The sum of a row of dS is 0 but for the rounding of y in delta: what comes out instead is the correction of delta that
   // the other kernel uses (gradients of keys in fp16: error 1.5 -> 1.4 times that of rounding the result alone).
   float rest = 0.f;
+  Range range;
   f32x16 acc[DP / 32];
 #pragma unroll
   for (int db = 0; db < DP / 32; ++db) acc[db] = f32x16{};
@@ -163,15 +231,8 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 && DMA && !(FIX && DP == 1
       for (int c = 0; c < DP / 16; ++c) mma(dp, L::row_frag(stage + kTile + row_at, kb, c), gf[c]);
       __builtin_amdgcn_sched_barrier(0);
       [[maybe_unused]] f32x16 pp;
-      const int first = t * KT + 32 * kb + 4 * (lane >> 5);
-#pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        const float e = exp2_fast(fmaf(p[i], sh.scale_log2, -base)), x = e * (dp[i] - delta);
-        const bool hidden = masked && first + block_row(i) >= lim;
-        if constexpr (FIX) pp[i] = hidden ? 0.f : e;
-        p[i] = hidden ? 0.f : x;
-        rest += p[i];
-      }
+      differences<T, FIX>(p, pp, dp, acc, rest, range, sh.scale_log2, base, delta, masked,
+                          t * KT + 32 * kb + 4 * (lane >> 5), lim);
       __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
@@ -186,6 +247,12 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 && DMA && !(FIX && DP == 1
     }
   }
   rest = halves_sum(rest);
+  if constexpr (kRanged<T>) {
+    const float f = kLower<T> / range.scale;
+    rest *= f;
+    settle(acc, f);
+    if constexpr (FIX) settle(pk, kLower<T>);
+  }
   if (valid && lane < 32) a.values[row] = {base, delta + rest};
   if constexpr (FIX) {
 #pragma unroll
@@ -197,11 +264,13 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 && DMA && !(FIX && DP == 1
 }
 
 // What 32 rows (their q at LDS address q_at, gy `to_g` further on, values at `in`) add to the gradients of the wavefront's 32
-// keys.  hidden: rows before it do not see the lane's key.
+// keys.  hidden: rows before it do not see the lane's key; live: the lane has a key (what the others compute is dropped, and
+// must not count for the range).
 template <typename T, int DP>
 __device__ inline void keys_block(f32x16 (&gk)[DP / 32], f32x16 (&gv)[DP / 32], const Frag<T> (&kf)[DP / 16],
                                   const Frag<T> (&vf)[DP / 16], uint32_t q_at, uint32_t to_g, uint32_t in, bool masked,
-                                  int hidden, float scale_log2, uint32_t row_at, uint32_t col_at, int lane) {
+                                  int hidden, bool live, Range &range, float scale_log2, uint32_t row_at, uint32_t col_at,
+                                  int lane) {
   typedef Tile<T, DP> L;
   const uint32_t g_at = q_at + to_g;
   in += (uint32_t)(4 * (lane >> 5) * 8);
@@ -239,8 +308,15 @@ __device__ inline void keys_block(f32x16 (&gk)[DP / 32], f32x16 (&gv)[DP / 32], 
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
       const int i = 2 * i2 + e;
-      dp[i] = p[i] == 0.f ? 0.f : p[i] * (dp[i] - pair[2 * e + 1]);
+      if constexpr (kRanged<T>) dp[i] = p[i] * range.scale * (dp[i] - pair[2 * e + 1]);  // finite, as fp16 operands are
+      else dp[i] = p[i] == 0.f ? 0.f : p[i] * (dp[i] - pair[2 * e + 1]);
     }
+  }
+  if constexpr (kRanged<T>) {
+    float m = 0.f;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) m = fmaxf(m, fabsf(dp[i]));
+    fit(range, dp, gk, live ? m : 0.f);
   }
   __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
@@ -304,6 +380,7 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 && DMA ? 2 : 1) void keys_
   lg_ = lq_;
   RowWalk walk((uint32_t)wg_first, sh);
   float value = 0.f;
+  Range range;
   // the tile of rows from r on, where the walk stands, into a stage; the values of a row side by side
   auto fetch = [&](int r, int stage_no) {
     const uint32_t stage = lds0 + (uint32_t)stage_no * 2 * kTile;
@@ -350,8 +427,12 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 && DMA ? 2 : 1) void keys_
 #pragma unroll 1
     for (int qb = 0; qb < QT / 32; ++qb) {
       keys_block<T, DP>(gk, gv, kf, vf, stage + (uint32_t)(qb * 32 * L::kPitch), kTile, values + (uint32_t)(qb * 32 * 8), masked,
-                        min(QT, my_first - r) - 32 * qb, sh.scale_log2, row_at, col_at, lane);
+                        min(QT, my_first - r) - 32 * qb, valid, range, sh.scale_log2, row_at, col_at, lane);
     }
+  }
+  if constexpr (kRanged<T>) {
+    settle(gk, kLower<T> / range.scale);
+    settle(gv, kLower<T>);
   }
   if (!exists) return;
   // the two gradients may be one tensor (the same tensor as keys and values): one after the other, by the same lane
@@ -467,11 +548,12 @@ __global__ __launch_bounds__(64 * W, 1) void few_queries_kernel(const BwArgs<T> 
   for (int s = 0; s < S; ++s) fetch(key + s * kStep, s);
 
   delta = halves_sum(delta);
-  const float base = valid ? row_base(a.stats[row]) : INFINITY;
+  const float base = valid ? row_base<T>(a.stats[row]) : INFINITY;
 
   arrived(qf);
   arrived(gf);
   float rest = 0.f;  // corrects delta, as in queries_kernel
+  Range range;
   f32x16 acc[DP / 32];
 #pragma unroll
   for (int db = 0; db < DP / 32; ++db) acc[db] = f32x16{};
@@ -498,15 +580,7 @@ __global__ __launch_bounds__(64 * W, 1) void few_queries_kernel(const BwArgs<T> 
     for (int c = 0; c < DP / 16; ++c) mma(dp, L::row_frag(stage + kTile + row_at, 0, c), gf[c]);
     const bool masked = key + 32 > all;
     [[maybe_unused]] f32x16 pp;
-    const int first = key + 4 * (lane >> 5);
-#pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      const float e = exp2_fast(fmaf(p[i], sh.scale_log2, -base)), x = e * (dp[i] - delta);
-      const bool hidden = masked && first + block_row(i) >= lim;
-      if constexpr (FIX) pp[i] = hidden ? 0.f : e;
-      p[i] = hidden ? 0.f : x;
-      rest += p[i];
-    }
+    differences<T, FIX>(p, pp, dp, acc, rest, range, sh.scale_log2, base, delta, masked, key + 4 * (lane >> 5), lim);
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
       const Frag<T> ds = as_operand(p, c, (Frag<T> *)nullptr);
@@ -524,6 +598,12 @@ __global__ __launch_bounds__(64 * W, 1) void few_queries_kernel(const BwArgs<T> 
   }
   wait_loads<0>();
   rest = halves_sum(rest);
+  if constexpr (kRanged<T>) {
+    const float f = kLower<T> / range.scale;
+    rest *= f;
+    settle(acc, f);
+    if constexpr (FIX) settle(pk, kLower<T>);
+  }
   if constexpr (W > 1) {
     __shared__ float rests[W][32];
     if (lane < 32) rests[wave][lane] = rest;
@@ -582,6 +662,7 @@ __global__ __launch_bounds__(64 * W, 1) void few_keys_kernel(const BwArgs<T> a) 
   lq_.init(sh.g, sh.hq * sh.d, sh.d, lane);
   lg_ = lq_;
   float value = 0.f;
+  Range range;
   int rr = first_row(k0) / 32 * 32 + 32 * wave;
   RowWalk walk((uint32_t)rr, sh);
   // the rows from `from` on, where the walk stands, into stage s; lane 2 i + e brings value e of row i
@@ -625,13 +706,18 @@ __global__ __launch_bounds__(64 * W, 1) void few_keys_kernel(const BwArgs<T> a) 
       *lds_ptr<float>(in + (uint32_t)lane * 4) = value;
       fetch(rr + kStep, 0);
     }
-    keys_block<T, DP>(gk, gv, kf, vf, stage, kTile, in, rr < all, my_first - rr, sh.scale_log2, row_at, col_at, lane);
+    keys_block<T, DP>(gk, gv, kf, vf, stage, kTile, in, rr < all, my_first - rr, valid, range, sh.scale_log2, row_at, col_at,
+                      lane);
     if constexpr (DMA) {
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the tile's reads are done before its place is filled again
       fetch(rr + S * kStep, s);
     }
   }
   wait_loads<0>();
+  if constexpr (kRanged<T>) {
+    settle(gk, kLower<T> / range.scale);
+    settle(gv, kLower<T>);
+  }
   auto in_k = [&](int i) { return i < exist ? a.gk + (row_0 + (size_t)i * sh.hk) * sh.d : (T *)nullptr; };
   auto in_v = [&](int i) { return i < exist ? a.gv + (row_0 + (size_t)i * sh.hk) * sh.d : (T *)nullptr; };
   // the two gradients may be one tensor: one after the other, by the same thread

@@ -187,6 +187,89 @@ def test_attention_of_one_tensor_with_tiles_of_128_rows(devices, kind):  # noqa:
     check("g", seen[0][1], total, tol)
 
 
+# fp16 holds 2^-24 .. 65504; probabilities of thousands of keys, and these times gradients, need not lie in it.
+# (queries, keys, heads, batch): few tiles, and tiles of 128 rows
+SCALED = {"few": (24, 6000, 2, 1), "large": (16, 4096, 8, 17)}
+
+
+@pytest.mark.parametrize("name", sorted(SCALED))
+@pytest.mark.parametrize("size_gy", (1e-2, 1e-3, 2e-4))
+@pytest.mark.parametrize("wide", ("q", "k"))
+def test_fp16_gradients_of_many_keys_lose_no_range(devices, wide, size_gy, name):  # noqa: F811
+    """gq and gk from a dS far below fp16's normal range, where gy and the gradients are in it.
+
+    dS = P (dP - delta) is rounded once for the matrix instructions, by at most h = 2^-11 of itself, with signs that are
+    independent of each other: what they add to an element of gq has a root mean square of at most
+    h scale sqrt(sum_j (dS k)^2), and likewise for gk.  The stored y (off by at most h of itself) adds an error to delta
+    whose root mean square is h sqrt(sum gy^2 y^2), and that, times P, one to dS; the result is rounded once (h of itself, or
+    half of fp16's smallest step, 2^-25).  fp32 roundings are 2^-12 of these.  All of these are upper bounds of the single
+    errors, so that the measured root mean square has to stay below their sum (in fact about 1 / sqrt(3) of it)."""
+    dev = devices["f16"]
+    n, m, heads, bs = SCALED[name]
+    d, scale, h = 64, 0.125, 2.0 ** -11
+    rng = np.random.default_rng(21)
+    q, k, v, gy = (draw(rng, "f16", bs, t, heads, d) for t in (n, m, m, n))
+    # scores of order 1, and the operand that the wanted gradient is a sum of is large: the gradient is in fp16's range
+    q, k = (rounded(x * (32.0 if wide == w else 1 / 32.0), "f16") for x, w in ((q, "q"), (k, "k")))
+    gy = rounded(gy * size_gy, "f16")
+    t = [tensor(dev, x) for x in (q, k, v, gy)]
+    dev.gemm_trace(True)
+    y, stats = dev.attention_fw(*t[:3], False, scale, None, stats=True)
+    g = [dev.new_tensor_by_constant(x.shape(), 0) for x in t[:3]]
+    dev.attention_bw(*t[:3], y, t[3], stats, False, scale, None, *g)
+    assert ("attention_queries" in dev.gemm_trace(False)) == (name == "large")
+    got = [x.to_vector().astype(np.float64).reshape(z.shape) for x, z in zip(g, (q, k, v))]
+    q, k, v, gy = (x.astype(np.float64) for x in (q, k, v, gy))
+    error, bound = [], []
+    for b in range(bs):
+        for a in range(heads):
+            Q, K, V, G = (x[b, :, a] for x in (q, k, v, gy))
+            P = np.exp(scale * Q @ K.T)
+            P /= P.sum(1, keepdims=True)
+            Y, dP = P @ V, G @ V.T
+            dS = P * (dP - (G * Y).sum(1)[:, None])
+            at_delta = P * (h * np.sqrt((G * G * Y * Y).sum(1)))[:, None]
+            if wide == "k":   # gq
+                want, parts = scale * dS @ K, scale * np.sqrt((dS * dS) @ (K * K))
+                delta = scale * np.abs(at_delta @ K)
+                error.append(got[0][b, :, a] - want)
+            else:             # gk
+                want, parts = scale * dS.T @ Q, scale * np.sqrt((dS * dS).T @ (Q * Q))
+                delta = scale * np.sqrt((at_delta * at_delta).T @ (Q * Q))
+                error.append(got[1][b, :, a] - want)
+            own = np.maximum(h * np.abs(want), 2.0 ** -25)
+            assert np.sqrt((want * want).mean()) > 2.0 ** -19, "the gradient itself is out of range"
+            bound.append(np.sqrt((h * parts) ** 2 + delta ** 2 + own ** 2))
+    error, bound = (np.sqrt((np.stack(x) ** 2).mean()) for x in (error, bound))
+    assert error <= bound, "%.3g, %.2f times the bound" % (error, error / bound)
+
+
+@pytest.mark.parametrize("name", ("few", "large"))
+def test_fp16_gradients_beyond_the_largest_number_on_the_way(devices, name):  # noqa: F811
+    """dS above 65504 where the gradients are below it."""
+    dev = devices["f16"]
+    rng = np.random.default_rng(22)
+    n, heads, bs = (40, 2, 1) if name == "few" else (70, 8, 35)
+    q, k, v, gy = (draw(rng, "f16", bs, n, heads, 64) for _ in range(4))
+    q, k, v, gy = (rounded(x * f, "f16") for x, f in ((q, 1 / 16), (k, 1 / 16), (v, 8), (gy, 6000)))
+    seqs = places(bs, n, n)
+    want = Attention(q, k, v, seqs, True, 0.125, "f16", gy)
+    t = [tensor(dev, x) for x in (q, k, v, gy)]
+    y, stats = dev.attention_fw(*t[:3], True, 0.125, None, stats=True)
+    g = [dev.new_tensor_by_constant(x.shape(), 0) for x in t[:3]]
+    dev.attention_bw(*t[:3], y, t[3], stats, True, 0.125, None, *g)
+    s = q[0, :, 0].astype(np.float64) @ k[0, :, 0].T * 0.125
+    p = np.where(np.tril(np.ones((n, n), bool)), np.exp(s), 0)
+    p /= p.sum(1, keepdims=True)
+    dp = gy[0, :, 0].astype(np.float64) @ v[0, :, 0].T
+    dS = np.abs(p * (dp - (p * dp).sum(1, keepdims=True))).max()
+    assert dS > 65504 > max(np.abs(want.gq).max(), np.abs(want.gk).max(), np.abs(want.gv).max())
+    # of a dS scaled so that the largest of a block is 2^12 or more, the smallest step is 2^-36 of that largest one
+    step = 2.0 ** -37 * 4 * dS * 0.125 * n * max(np.abs(q).max(), np.abs(k).max())
+    for x, r in zip(g, ("gq", "gk", "gv")):
+        check(r, x.to_vector(), getattr(want, r), getattr(want, "tol_" + r) + (step if r != "gv" else 0))
+
+
 @pytest.mark.parametrize("name,shape", (("few", (4, 2, 4096, 1)), ("split", (1, 1, 8192, 1)), ("large", (130, 8, 1500, 18))))
 def test_fp16_many_small_probabilities_beside_a_large_one(devices, name, shape):  # noqa: F811
     """One key takes nearly all of the weight, with a value of zero: the result is what thousands of keys with weights of
