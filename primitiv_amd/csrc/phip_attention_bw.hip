@@ -129,9 +129,18 @@ constexpr int kKeys = sizeof(T) == 2 ? 64 : 32;
 // gq and delta: the loop of the forward kernel with P recomputed instead of the running softmax.
 //
 // delta comes from y as it was stored.  In 16-bit storage its rounding is an error e of delta that adds -e P k to gq, and with
-// few keys per row that shows (sequences of 6 to 19 tokens in bf16: gq 1.65 times as far off as its own rounding).  FIX adds
-// up P k as well, one more product on the fragments at hand, and takes e, which is minus the sum of a row of dS, back out:
-// for 16-bit storage and fewer than 1024 keys; behind that the error is lost among those of more terms (8192 keys: 1.4 times).
+// few keys per row that shows.  FIX adds up P k as well, one more product on the fragments at hand, and takes e, which is minus
+// the sum of a row of dS, back out.  Root mean square error of gq in units of that of rounding gq alone, and time of a training
+// step on 32 Ki tokens (causal, bf16, 16 heads of 64 / 16 over 4 of 128; fp16 alike):
+//   keys           8     16     32         64          128         512         1023
+//   error without  1.82  1.72   1.65       1.59        1.54        1.52        1.50
+//   error with     1.41  1.42   1.43       1.43        1.42        1.42        1.42
+//   us without           1008 / 684  592 / 475  359 / 526  346 / 474  439 / 614  575 / 897
+//   us with              1190 / 893  674 / 552  390 / 632  344 / 608  459 / 785  618 / 1152
+// With heads of 128 the sums of P k cost the second workgroup per CU, so FIX is taken up to 64 keys, where it takes a tenth of
+// the error.
+constexpr uint64_t kFixKeys = 64;
+
 template <typename T, int DP, bool DMA, bool FIX>
 __global__ __launch_bounds__(kThreads, sizeof(T) == 2 && DMA && !(FIX && DP == 128) ? 2 : 1) void queries_kernel(const BwArgs<T> a) {
   constexpr int KT = kKeys<T>, BM = 32 * kWaves;
@@ -755,7 +764,7 @@ int launch(phip_ctx *ctx, BwArgs<T> a, const phip_sequences *seqs) {
     return launch_kernel<queries_kernel<T, DP, DMA, FIX>>(ctx, FIX ? "attention_queries_fix" : "attention_queries", a, wide_q, kThreads, lds_q);
   };
   int rc = PHIP_OK;
-  if constexpr (sizeof(T) == 2) rc = most_k < 1024 ? queries(std::true_type()) : queries(std::false_type());
+  if constexpr (sizeof(T) == 2) rc = most_k <= kFixKeys ? queries(std::true_type()) : queries(std::false_type());
   else rc = queries(std::false_type());
   if (rc != PHIP_OK) return rc;
   a.tiles = (uint32_t)(way_k == Way::Shared ? (keys + 127) / 128 : (keys + 31) / 32);

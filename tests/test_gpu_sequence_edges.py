@@ -100,6 +100,8 @@ def attention_against_reference(dev, kind, shape, seed, kernels):
     dev.attention_bw(tq_, tk_, tv_, y, tg_, stats, causal, scale, lists, g["gq"], g["gk"], g["gv"])
     went = dev.gemm_trace(False)
     assert [w.replace("_fix", "") for w in went] == list(kernels), went
+    # the rounding of y in delta is taken out for 16-bit storage and up to 64 keys
+    assert went[1].endswith("_fix") == (kind != "f32" and max(k_lens or q_lens or (tk,)) <= 64)
     check("y", y.to_vector(), want.y, want.tol_y)
     got = stats.to_vector().reshape(want.stats.shape)
     assert np.array_equal(np.isneginf(got), np.isneginf(want.stats))
@@ -121,6 +123,22 @@ def test_attention_with_tiles_of_128_rows(devices, kind, name):  # noqa: F811
     """The kernels whose workgroups share tiles, which prompts and training go to."""
     attention_against_reference(devices[kind], kind, LARGE[name], 30 + len(name),
                                 ("attention_rows", "attention_queries", "attention_keys"))
+
+
+# Up to 64 keys: 16-bit storage takes the rounding of the stored result out of the queries' gradients
+FEW_KEYS = {
+    "size_64": (64, 16, 8, 150, 64, 40, None, None, False, False),
+    "size_65": (65, 8, 8, 130, 50, 40, None, None, False, True),
+    "size_128": (128, 8, 8, 70, 64, 40, (70, 0, 1, 64) * 10, (64, 33, 1, 64) * 10, False, True),
+}
+
+
+@pytest.mark.parametrize("name", sorted(FEW_KEYS))
+@pytest.mark.parametrize("kind", KINDS[1:])
+def test_attention_with_tiles_of_128_rows_and_few_keys(devices, kind, name):  # noqa: F811
+    went = attention_against_reference(devices[kind], kind, FEW_KEYS[name], 50 + len(name),
+                                       ("attention_rows", "attention_queries", "attention_keys"))
+    assert went[1] == "attention_queries_fix"
 
 
 # Short sequences, so many that every SIMD has one: in fp32 a wavefront each
