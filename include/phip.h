@@ -739,8 +739,9 @@ int phip_norm_rotary_bw_bf16(phip_ctx *ctx, const void *xq, const void *xk, cons
  * split the keys between workgroups.
  * Backward: gq, gk, gv += from q, k, v, the forward call's y and stats, and
  * gy; the heads that share a key head add up in its gradient.  One tensor may
- * be queries, keys and values: its gradient is then passed for each.  All sums
- * are in fp32 and in a fixed order: the same bits on every run. */
+ * be queries, keys and values: its gradient is then passed for each (hq == hk
+ * and tq == tk where it is that of queries too); gradients overlap in no other
+ * way.  All sums are in fp32 and in a fixed order: the same bits on every run. */
 int phip_attention_fw_f32(phip_ctx *ctx, const float *q, const float *k, const float *v, float *y, float *stats,
     uint32_t d, uint32_t hq, uint32_t hk, uint32_t tq, uint32_t tk, uint32_t bs, const phip_sequences *seqs,
     int causal, float scale);

@@ -806,10 +806,10 @@ int backward(phip_ctx *ctx, const T *q, const T *k, const T *v, const T *y, cons
   };
   PHIP_REQUIRE(!is_read(gq, nq) && !is_read(gk, nk) && !is_read(gv, nk), "a gradient shares memory with an operand");
   // the same tensor may be queries, keys and values, and then its one gradient is passed for each; anything in between
-  // would have two lanes add to one element
-  PHIP_REQUIRE((gk == gv || !shares_memory(gk, nk, gv, nk)) &&
-                   ((const void *)gq == gk || !shares_memory(gq, nq, gk, nk)) &&
-                   ((const void *)gq == gv || !shares_memory(gq, nq, gv, nk)),
+  // would have two lanes add to one element, or two layouts in one tensor
+  const bool alike = hq == hk && tq == tk;
+  PHIP_REQUIRE((gk == gv || !shares_memory(gk, nk, gv, nk)) && (gq == gk ? alike : !shares_memory(gq, nq, gk, nk)) &&
+                   (gq == gv ? alike : !shares_memory(gq, nq, gv, nk)),
                "two gradients overlap without being the same tensor");
   PHIP_REQUIRE(slots(a.seq, 32, a.s.g, false) * hk < 0x7fffffffu && slots(a.seq, 32, 1, true) * hk < 0x7fffffffu, "too many rows");
   void *values = nullptr;

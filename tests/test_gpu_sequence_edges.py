@@ -1,9 +1,12 @@
 """Sequence operators where their inputs, sizes or addresses are unusual: against the plain 64-bit forms, with bounds counted
 from the roundings (sequence_reference.py)."""
+import ctypes
+
 import numpy as np
 import pytest
 
 import primitiv_amd as pa
+from primitiv_amd import _lib
 from sequence_reference import Attention, HALF, Rotary, TINY, places
 from test_gpu_sequence_operators import KINDS, check, devices, draw, rounded, tensor  # noqa: F401
 
@@ -308,3 +311,22 @@ def test_fp16_many_small_probabilities_beside_a_large_one(devices, name, shape):
     # two halves of a step; scores of 18 are off by 70 x 2^-24 x 18 at most
     check("y", y.to_vector(), want.y, np.abs(want.y) * (2 * 2.0 ** -11 + 2.0 ** -13) + 2.0 ** -25)
     check("stats", stats.to_vector(), want.stats.reshape(-1), want.tol_stats.reshape(-1))
+
+
+def test_one_gradient_for_operands_of_different_shapes_is_refused(devices):  # noqa: F811
+    """The gradient of queries is that of keys (or values) only where they have the same heads and tokens."""
+    dev = devices["f32"]
+    ones = lambda n: dev.new_tensor_by_constant(S([n]), 1)  # noqa: E731
+    for hq, hk, tq, tk in ((4, 2, 6, 6), (2, 2, 6, 7), (2, 2, 7, 6), (4, 4, 6, 6)):
+        q, k, y, g, other = ones(64 * hq * tq), ones(64 * hk * tk), ones(64 * hq * tq), ones(64 * 4 * 8), ones(64 * 4 * 8)
+        stats = ones(hq * tq)
+        for gq, gk, gv in ((g, g, other), (g, other, g), (g, g, g), (other, g, g)):
+            before = [x.to_vector() for x in (g, other)]
+            rc = _lib.lib().phip_attention_bw_f32(
+                dev.ctx(), q.handle(), k.handle(), k.handle(), y.handle(), stats.handle(), y.handle(), gq.handle(), gk.handle(),
+                gv.handle(), 64, hq, hk, tq, tk, 1, None, 1, 0.125)
+            if (hq, tq) == (hk, tk) or gq is other:
+                assert rc == _lib.PHIP_OK
+            else:
+                assert rc == _lib.PHIP_ERR_INVALID_ARGUMENT and b"overlap" in _lib.lib().phip_last_error()
+                assert all(np.array_equal(a, x.to_vector()) for a, x in zip(before, (g, other)))
