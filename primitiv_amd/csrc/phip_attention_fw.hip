@@ -616,10 +616,15 @@ int forward(phip_ctx *ctx, const T *q, const T *k, const T *v, T *y, float *stat
   rc = sequence_view(ctx, seqs, tq, tk, bs, true, &a.seq);
   if (rc != PHIP_OK) return rc;
   PHIP_REQUIRE(q != nullptr && k != nullptr && v != nullptr && y != nullptr, "null pointer");
-  PHIP_REQUIRE(elements_aligned(sizeof(T), {q, k, v, y}), "an address is no multiple of the element size");
+  PHIP_REQUIRE(elements_aligned(sizeof(T), {q, k, v, y}) && elements_aligned(4, {stats}),
+               "an address is no multiple of the element size");
   const size_t ny = (size_t)d * hq * tq * bs * sizeof(T), nk = (size_t)d * hk * tk * bs * sizeof(T);
+  const size_t ns = (size_t)hq * tq * bs * sizeof(float);
   PHIP_REQUIRE(!shares_memory(y, ny, q, ny) && !shares_memory(y, ny, k, nk) && !shares_memory(y, ny, v, nk),
                "the result shares memory with an operand");
+  PHIP_REQUIRE(stats == nullptr || (!shares_memory(stats, ns, q, ny) && !shares_memory(stats, ns, k, nk) &&
+                                    !shares_memory(stats, ns, v, nk) && !shares_memory(stats, ns, y, ny)),
+               "stats share memory with an operand or the result");
   a.q = q;
   a.k = k;
   a.v = v;

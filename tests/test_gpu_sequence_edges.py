@@ -330,3 +330,19 @@ def test_one_gradient_for_operands_of_different_shapes_is_refused(devices):  # n
             else:
                 assert rc == _lib.PHIP_ERR_INVALID_ARGUMENT and b"overlap" in _lib.lib().phip_last_error()
                 assert all(np.array_equal(a, x.to_vector()) for a, x in zip(before, (g, other)))
+
+
+def test_stats_in_another_tensor_or_at_an_odd_address_are_refused(devices):  # noqa: F811
+    dev = devices["f32"]
+    q, k, v, y = (dev.new_tensor_by_constant(S([64, h, 6], 2), 1) for h in (4, 2, 2, 4))
+    own = dev.new_tensor_by_constant(S([4 * 6 * 2 + 4]), 5)
+    call = lambda stats: _lib.lib().phip_attention_fw_f32(  # noqa: E731
+        dev.ctx(), q.handle(), k.handle(), v.handle(), y.handle(), stats, 64, 4, 2, 6, 6, 2, None, 1, 0.125)
+    for x in (q, k, v, y):
+        for stats in (x.handle(), x.handle() + 4 * (x.shape().size() - 1), x.handle() - 4 * 47):
+            assert call(stats) == _lib.PHIP_ERR_INVALID_ARGUMENT and b"share" in _lib.lib().phip_last_error()
+    for o in (1, 2, 3):
+        assert call(own.handle() + o) == _lib.PHIP_ERR_INVALID_ARGUMENT and b"multiple" in _lib.lib().phip_last_error()
+    assert all((x.to_vector() == c).all() for x, c in ((q, 1), (k, 1), (v, 1), (y, 1), (own, 5)))
+    assert call(own.handle() + 4) == _lib.PHIP_OK
+    assert (own.to_vector()[[0, -3, -2, -1]] == 5).all() and (own.to_vector()[1:-3] != 5).all()
