@@ -10,6 +10,7 @@
 // are computed once per token into LDS.  A row is spread over the fewest lanes that hold it at two 16-byte chunks each, one
 // for either side of its pairs, so a pair never leaves its lane and the norm is a few exchanges between neighbours.
 #include <algorithm>
+#include <initializer_list>
 
 #include "phip_pointwise.h"
 #include "phip_sequences.h"
@@ -356,6 +357,9 @@ int make_args(phip_ctx *ctx, uint32_t d, uint32_t hq, uint32_t hk, uint32_t t, u
 }
 
 inline bool aligned(const void *p, size_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
+inline bool all_aligned(size_t n, std::initializer_list<const void *> ptrs) {
+  return std::all_of(ptrs.begin(), ptrs.end(), [n](const void *p) { return aligned(p, n); });
+}
 
 template <typename T, int V, bool INTER, bool NORM, bool BACK>
 int launch_kernel(phip_ctx *ctx, Args<T> a) {
@@ -408,6 +412,7 @@ int forward(phip_ctx *ctx, const T *xq, const T *xk, const T *wq, const T *wk, T
   if (rc != PHIP_OK) return rc;
   PHIP_REQUIRE(xq != nullptr && yq != nullptr && (xk == nullptr) == (yk == nullptr), "null pointer");
   PHIP_REQUIRE(!NORM || (wq != nullptr && (xk == nullptr) == (wk == nullptr)), "null weights");
+  PHIP_REQUIRE(all_aligned(sizeof(T), {xq, xk, wq, wk, yq, yk}), "an address is no multiple of the element size");
   const size_t nq = (size_t)d * hq * a.tokens * sizeof(T), nk = (size_t)d * hk * a.tokens * sizeof(T);
   auto read = [&](const void *y, size_t n) {
     return shares_memory(y, n, wq, d * sizeof(T)) || shares_memory(y, n, wk, d * sizeof(T)) ||
@@ -451,6 +456,8 @@ int backward(phip_ctx *ctx, const T *xq, const T *xk, const T *wq, const T *wk, 
   PHIP_REQUIRE(!NORM || (xq != nullptr && wq != nullptr && gwq != nullptr && has_k == (xk != nullptr) &&
                          has_k == (wk != nullptr) && has_k == (gwk != nullptr)),
                "null operand, weights or gradient of the weights");
+  PHIP_REQUIRE(all_aligned(sizeof(T), {xq, xk, wq, wk, gyq, gyk, gxq, gxk, gwq, gwk}),
+               "an address is no multiple of the element size");
   const size_t nq = (size_t)d * hq * a.tokens * sizeof(T), nk = (size_t)d * hk * a.tokens * sizeof(T), nw = d * sizeof(T);
   auto is_read = [&](const void *g, size_t n) {
     return shares_memory(g, n, xq, nq) || shares_memory(g, n, xk, nk) || shares_memory(g, n, wq, nw) ||

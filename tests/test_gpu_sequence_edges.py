@@ -346,3 +346,22 @@ def test_stats_in_another_tensor_or_at_an_odd_address_are_refused(devices):  # n
     assert all((x.to_vector() == c).all() for x, c in ((q, 1), (k, 1), (v, 1), (y, 1), (own, 5)))
     assert call(own.handle() + 4) == _lib.PHIP_OK
     assert (own.to_vector()[[0, -3, -2, -1]] == 5).all() and (own.to_vector()[1:-3] != 5).all()
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_rotary_at_an_odd_address_is_refused(devices, kind):  # noqa: F811
+    dev = devices[kind]
+    f = (ctypes.c_float * 32)()
+    size = 64 * 2 * 5
+    block = dev.new_tensor_by_constant(S([8 * size]), 1)
+    rest = (64, 2, 2, 5, 1, None, 0, f, 32, 0, 1.0)
+    for norm in (False, True):
+        for back in (False, True):
+            n = (10 if norm else 4) if back else (6 if norm else 4)
+            name = "phip_%srotary_%s_%s" % ("norm_" if norm else "", "bw" if back else "fw", kind)
+            good = [block.handle() + dev._ITEMSIZE * (size * i if i < 6 else 6 * size + 64 * i) for i in range(n)]
+            for odd in range(n):
+                args = [p + (1 if i == odd else 0) for i, p in enumerate(good)]
+                rc = getattr(_lib.lib(), name)(dev.ctx(), *args, *rest, *((1e-6,) if norm else ()))
+                assert rc == _lib.PHIP_ERR_INVALID_ARGUMENT and b"multiple" in _lib.lib().phip_last_error(), (name, odd)
+    assert (block.to_vector() == 1).all()
