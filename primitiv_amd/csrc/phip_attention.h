@@ -555,6 +555,8 @@ inline Way choose_way(phip_ctx *ctx, uint64_t wide, uint64_t narrow, uint64_t mo
 }
 
 constexpr uint32_t kMostSize = 128;  // largest head size
+// A launch has fewer than 2^32 threads.
+inline bool launchable(uint64_t blocks, uint64_t threads) { return blocks < (1ull << 32) / threads; }
 
 // Checks what the forward and the gradient calls have in common.
 inline int make_shape(uint32_t d, uint32_t hq, uint32_t hk, uint32_t tq, uint32_t tk, uint32_t bs, int causal, float scale,

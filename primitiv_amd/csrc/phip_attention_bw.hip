@@ -744,44 +744,71 @@ int launch_kernel(phip_ctx *ctx, const char *name, const BwArgs<T> &a, uint64_t 
   return PHIP_OK;
 }
 
+// The workgroups of the two kernels.
+struct Plan {
+  struct Side {
+    Way way;
+    uint64_t wide, narrow;  // with tiles of 128, of 32
+    bool launchable() const {
+      return way == Way::Shared ? attention::launchable(wide, kThreads) : attention::launchable(narrow, way == Way::One ? 64 : 256);
+    }
+  };
+  Side q, k;
+  uint64_t most_k;          // keys of the longest sequence
+};
+
+template <typename T>
+Plan make_plan(phip_ctx *ctx, const BwArgs<T> &a, const phip_sequences *seqs) {
+  const uint64_t most_q = (uint64_t)(seqs != nullptr ? seqs->max_q : a.seq.tq) * a.s.g, most_k = seqs != nullptr ? seqs->max_k : a.seq.tk;
+  Plan p = {{Way::Shared, slots(a.seq, 128, a.s.g, false) * a.s.hk, slots(a.seq, 32, a.s.g, false) * a.s.hk},
+            {Way::Shared, slots(a.seq, 128, 1, true) * a.s.hk, slots(a.seq, 32, 1, true) * a.s.hk},
+            most_k};
+  p.q.way = choose_way<T>(ctx, p.q.wide, p.q.narrow, most_q, most_k);
+  p.k.way = choose_way<T>(ctx, p.k.wide, p.k.narrow, most_k, most_q);
+  return p;
+}
+
 template <typename T, int DP, bool DMA>
-int launch(phip_ctx *ctx, BwArgs<T> a, const phip_sequences *seqs) {
+int launch(phip_ctx *ctx, BwArgs<T> a, const Plan &plan) {
   constexpr int lds_q = 4 * kKeys<T> * Tile<T, DP>::kPitch;
   constexpr int lds_k = 4 * kRows<T> * Tile<T, DP>::kPitch + 4 * kRows<T> * 4;
-  const uint64_t most_q = (uint64_t)(seqs != nullptr ? seqs->max_q : a.seq.tq) * a.s.g, most_k = seqs != nullptr ? seqs->max_k : a.seq.tk;
-  const uint64_t wide_q = slots(a.seq, 128, a.s.g, false) * a.s.hk, narrow_q = slots(a.seq, 32, a.s.g, false) * a.s.hk;
-  const uint64_t wide_k = slots(a.seq, 128, 1, true) * a.s.hk, narrow_k = slots(a.seq, 32, 1, true) * a.s.hk;
-  const Way way_q = choose_way<T>(ctx, wide_q, narrow_q, most_q, most_k), way_k = choose_way<T>(ctx, wide_k, narrow_k, most_k, most_q);
+  const Way way_q = plan.q.way, way_k = plan.k.way;
   const uint64_t rows = (uint64_t)a.seq.tq * a.s.g, keys = a.seq.tk;
   a.tiles = (uint32_t)(way_q == Way::Shared ? (rows + 127) / 128 : (rows + 31) / 32);
   auto queries = [&](auto fix) {
     constexpr bool FIX = decltype(fix)::value;
     if (way_q == Way::Four)
-      return launch_kernel<few_queries_kernel<T, DP, DMA, 4, FIX>>(ctx, FIX ? "attention_few_queries_fix" : "attention_few_queries", a, narrow_q, 256, kFewLds<T, DP, 4>);
+      return launch_kernel<few_queries_kernel<T, DP, DMA, 4, FIX>>(
+          ctx, FIX ? "attention_few_queries_fix" : "attention_few_queries", a, plan.q.narrow, 256, kFewLds<T, DP, 4>);
     if constexpr (sizeof(T) == 4) {
-      if (way_q == Way::One) return launch_kernel<few_queries_kernel<T, DP, DMA, 1, FIX>>(ctx, "attention_few1_queries", a, narrow_q, 64, kFewLds<T, DP, 1>);
+      if (way_q == Way::One)
+        return launch_kernel<few_queries_kernel<T, DP, DMA, 1, FIX>>(ctx, "attention_few1_queries", a, plan.q.narrow, 64,
+                                                                     kFewLds<T, DP, 1>);
     }
-    return launch_kernel<queries_kernel<T, DP, DMA, FIX>>(ctx, FIX ? "attention_queries_fix" : "attention_queries", a, wide_q, kThreads, lds_q);
+    return launch_kernel<queries_kernel<T, DP, DMA, FIX>>(ctx, FIX ? "attention_queries_fix" : "attention_queries", a,
+                                                          plan.q.wide, kThreads, lds_q);
   };
   int rc = PHIP_OK;
-  if constexpr (sizeof(T) == 2) rc = most_k <= kFixKeys ? queries(std::true_type()) : queries(std::false_type());
+  if constexpr (sizeof(T) == 2) rc = plan.most_k <= kFixKeys ? queries(std::true_type()) : queries(std::false_type());
   else rc = queries(std::false_type());
   if (rc != PHIP_OK) return rc;
   a.tiles = (uint32_t)(way_k == Way::Shared ? (keys + 127) / 128 : (keys + 31) / 32);
-  if (way_k == Way::Four) return launch_kernel<few_keys_kernel<T, DP, DMA, 4>>(ctx, "attention_few_keys", a, narrow_k, 256, kFewLds<T, DP, 4>);
+  if (way_k == Way::Four)
+    return launch_kernel<few_keys_kernel<T, DP, DMA, 4>>(ctx, "attention_few_keys", a, plan.k.narrow, 256, kFewLds<T, DP, 4>);
   if constexpr (sizeof(T) == 4) {
-    if (way_k == Way::One) return launch_kernel<few_keys_kernel<T, DP, DMA, 1>>(ctx, "attention_few1_keys", a, narrow_k, 64, kFewLds<T, DP, 1>);
+    if (way_k == Way::One)
+      return launch_kernel<few_keys_kernel<T, DP, DMA, 1>>(ctx, "attention_few1_keys", a, plan.k.narrow, 64, kFewLds<T, DP, 1>);
   }
-  return launch_kernel<keys_kernel<T, DP, DMA>>(ctx, "attention_keys", a, wide_k, kThreads, lds_k);
+  return launch_kernel<keys_kernel<T, DP, DMA>>(ctx, "attention_keys", a, plan.k.wide, kThreads, lds_k);
 }
 
 template <typename T, bool DMA>
-int dispatch(phip_ctx *ctx, const BwArgs<T> &a, const phip_sequences *seqs) {
+int dispatch(phip_ctx *ctx, const BwArgs<T> &a, const Plan &plan) {
   switch ((a.s.d + 31) / 32) {
-    case 1: return launch<T, 32, DMA>(ctx, a, seqs);
-    case 2: return launch<T, 64, DMA>(ctx, a, seqs);
-    case 3: return launch<T, 96, DMA>(ctx, a, seqs);
-    default: return launch<T, 128, DMA>(ctx, a, seqs);
+    case 1: return launch<T, 32, DMA>(ctx, a, plan);
+    case 2: return launch<T, 64, DMA>(ctx, a, plan);
+    case 3: return launch<T, 96, DMA>(ctx, a, plan);
+    default: return launch<T, 128, DMA>(ctx, a, plan);
   }
 }
 
@@ -811,7 +838,8 @@ int backward(phip_ctx *ctx, const T *q, const T *k, const T *v, const T *y, cons
   PHIP_REQUIRE((gk == gv || !shares_memory(gk, nk, gv, nk)) && (gq == gk ? alike : !shares_memory(gq, nq, gk, nk)) &&
                    (gq == gv ? alike : !shares_memory(gq, nq, gv, nk)),
                "two gradients overlap without being the same tensor");
-  PHIP_REQUIRE(slots(a.seq, 32, a.s.g, false) * hk < 0x7fffffffu && slots(a.seq, 32, 1, true) * hk < 0x7fffffffu, "too many rows");
+  const Plan plan = make_plan<T>(ctx, a, seqs);
+  PHIP_REQUIRE(plan.q.launchable() && plan.k.launchable(), "too many rows");
   void *values = nullptr;
   rc = phip_pool_alloc(ctx, 2 * ns, &values, nullptr);
   if (rc != PHIP_OK) return rc;
@@ -838,9 +866,9 @@ int backward(phip_ctx *ctx, const T *q, const T *k, const T *v, const T *y, cons
   bool dma = true;
   if constexpr (sizeof(T) == 2) {
     dma = rows_aligned(d, sizeof(T), 4, {q, k, v, gy});
-    if (!dma) rc = dispatch<T, false>(ctx, a, seqs);
+    if (!dma) rc = dispatch<T, false>(ctx, a, plan);
   }
-  if (dma) rc = dispatch<T, true>(ctx, a, seqs);
+  if (dma) rc = dispatch<T, true>(ctx, a, plan);
   phip_pool_free(ctx, values);
   return rc;
 }

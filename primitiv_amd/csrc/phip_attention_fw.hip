@@ -536,7 +536,7 @@ int launch_rows(phip_ctx *ctx, FwArgs<T> a) {
   constexpr int lds = 4 * kKeys<T> * Tile<T, DP>::kPitch;
   a.tiles = (uint32_t)(((uint64_t)a.seq.tq * a.s.g + BM - 1) / BM);
   const uint64_t blocks = slots(a.seq, BM, a.s.g, false) * a.s.hk;
-  PHIP_REQUIRE(blocks < 0x7fffffffu, "too many rows");
+  PHIP_REQUIRE(launchable(blocks, kThreads), "too many rows");
   const int rc = allow_lds<rows_kernel<T, DP, DMA>>(ctx, lds);
   if (rc != PHIP_OK) return rc;
   hipLaunchKernelGGL((rows_kernel<T, DP, DMA>), dim3((uint32_t)blocks), dim3(kThreads), lds, ctx->stream, a);
@@ -567,7 +567,7 @@ int launch_few(phip_ctx *ctx, FwArgs<T> a, const phip_sequences *seqs) {
   const uint32_t most = seqs != nullptr ? seqs->max_k : a.seq.tk;
   a.chunk = W == 1 ? most + 1 : few_chunk(ctx, a.seq, seqs, tiles);
   a.splits = most <= a.chunk ? 1 : (most + a.chunk - 1) / a.chunk;
-  PHIP_REQUIRE(tiles * a.splits < 0x7fffffffu, "too many rows");
+  PHIP_REQUIRE(launchable(tiles * a.splits, 64 * W), "too many rows");
   void *partial = nullptr;
   if (a.splits > 1) {
     const int rc2 = phip_pool_alloc(ctx, (size_t)tiles * a.splits * 32 * (DP + 4) * sizeof(float), &partial, nullptr);

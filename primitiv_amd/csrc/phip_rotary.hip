@@ -390,13 +390,14 @@ int launch(phip_ctx *ctx, const Args<T> &a, bool interleaved) {
 }
 
 // Tokens per step of a side's workgroups: as many as leave a few workgroups for every CU.  looping: every workgroup leaves
-// a row of partial sums, so their number is limited and they take several steps.
+// a row of partial sums, so their number is limited and they take several steps; without sums, a launch's 2^32 threads are
+// the limit.
 template <typename T>
 void choose(phip_ctx *ctx, Args<T> *a, bool looping) {
   const uint64_t cus = (uint64_t)ctx->prop.multiProcessorCount;
   for (Side<T> &s : a->side) {
     if (s.heads == 0) continue;
-    const uint64_t tt = a->tokens / (cus * 8), blocks_cap = looping ? cus * 4 : ~0ull;
+    const uint64_t tt = a->tokens / (cus * 8), blocks_cap = looping ? cus * 4 : 1u << 23;
     s.tt = (uint32_t)(tt < 1 ? 1 : tt > kMostTokens ? kMostTokens : tt);
     s.blocks = (uint32_t)std::min<uint64_t>((a->tokens + s.tt - 1) / s.tt, blocks_cap);
   }

@@ -365,3 +365,62 @@ def test_rotary_at_an_odd_address_is_refused(devices, kind):  # noqa: F811
                 rc = getattr(_lib.lib(), name)(dev.ctx(), *args, *rest, *((1e-6,) if norm else ()))
                 assert rc == _lib.PHIP_ERR_INVALID_ARGUMENT and b"multiple" in _lib.lib().phip_last_error(), (name, odd)
     assert (block.to_vector() == 1).all()
+
+
+def test_rotary_of_more_tokens_than_a_launch_has_threads_for():
+    """2^27 tokens and a few: 256 threads for every eight of them would be more than 2^32."""
+    dev = pa.HIP16(0, storage="f16")
+    tokens = 2 ** 27 + 13
+    x = dev.new_tensor_by_constant(S([2, 1, tokens]), 1)
+    freqs = np.float32([2.0 ** -10])
+    y, _ = dev.rotary_fw(x, None, freqs)
+    g = dev.new_tensor_by_constant(x.shape(), 0)
+    dev.rotary_bw(x, None, freqs, False, 0, 1.0, None, g, None)
+    for at in (0, 1000, 2 ** 26 + 5, 2 ** 27 - 3, tokens - 8):
+        p = (np.arange(at, at + 8) * float(freqs[0]))
+        for t, sign in ((y, 1), (g, -1)):
+            got = np.empty(16, np.float16)
+            _lib.call("phip_memcpy_d2h", dev.ctx(), got.ctypes.data, t.handle() + 4 * at, 32)
+            want = np.stack([np.cos(p) - sign * np.sin(p), np.cos(p) + sign * np.sin(p)], 1)
+            # fp32 cosines and sines (8 x 2^-24 of a sum of at most 2) and one rounding
+            check("at %d" % at, got, want, 2.0 ** -11 * np.abs(want) + 2.0 ** -20 + TINY["f16"])
+    del x, y, g
+    dev.close()
+
+
+def test_attention_of_more_sequences_than_a_launch_has_threads_for_is_refused():
+    dev = pa.HIP16(0, storage="f16")
+    n = 2 ** 24
+    x = dev.new_tensor_by_constant(S([1, 1, 1], n), 1)
+    with pytest.raises(pa.Error, match="too many rows"):
+        dev.attention_fw(x, x, x)
+    y, stats = dev.attention_fw(*(dev.new_tensor_by_constant(S([1, 1, 1], n - 1), 1) for _ in range(3)), stats=True)
+    assert (y.to_vector() == 1).all()
+    big = dev.new_tensor_by_constant(S([n]), 1)
+    g = dev.new_tensor_by_constant(x.shape(), 0)
+    rc = _lib.lib().phip_attention_bw_f16(dev.ctx(), x.handle(), x.handle(), x.handle(), x.handle(), _pool(dev, 4 * n), big.handle(),
+                                          g.mutable_handle(), g.mutable_handle(), g.mutable_handle(), 1, 1, 1, 1, 1, n, None, 1, 1.0)
+    assert rc == _lib.PHIP_ERR_INVALID_ARGUMENT and b"too many rows" in _lib.lib().phip_last_error()
+    assert (g.to_vector() == 0).all()   # a gradient that was to be zero is
+    del x, y, stats, big, g
+    dev.close()
+
+
+def _pool(dev, size):
+    ptr = ctypes.c_void_p()
+    _lib.call("phip_pool_alloc", dev.ctx(), size, ctypes.byref(ptr), None)
+    return ptr.value
+
+
+def test_attention_of_very_many_fp32_sequences():
+    """In fp32 short sequences take a wavefront each: four times as many as workgroups of four wavefronts could be."""
+    dev = pa.HIP(0)
+    n = 2 ** 24 + 5
+    q, k, v = (dev.new_tensor_by_constant(S([1, 1, 1], n), x) for x in (1, 2, 3))
+    y, stats = dev.attention_fw(q, k, v, scale=0.5, stats=True)
+    g = [dev.new_tensor_by_constant(q.shape(), 0) for _ in range(3)]
+    dev.attention_bw(q, k, v, y, v, stats, True, 0.5, None, *g)
+    for t, want in ((y, 3), (stats, 1), (g[0], 0), (g[1], 0), (g[2], 3)):
+        assert (t.to_vector() == want).all()
+    del q, k, v, y, stats, g
+    dev.close()
