@@ -23,9 +23,12 @@ struct FwArgs {
   SequenceView seq;
   uint32_t tiles;       // row tiles of a whole sample
   uint32_t vec_y;       // y's rows are aligned to four elements
-  // key ranges (few rows): keys per range, ranges, partial results
-  uint32_t chunk, splits;
-  float *partial;       // per tile and range: rows x DP sums, then rows maxima, rows sums
+  // key ranges (few rows): keys per range, partial results
+  uint32_t chunk;
+  uint32_t splits;      // ranges of the longest sequence; a workgroup for each range of each tile, or,
+  uint32_t listed;      // if not 0: workgroups for the ranges that the listed sequences have (see find_range): their slots
+  uint32_t part_rows;   // rows of a tile that exist at most
+  float *partial;       // per tile and range: part_rows x (DP sums, maximum, sum, 2 unused)
   uint32_t *tickets;
 };
 
@@ -321,6 +324,45 @@ __device__ inline bool last_of_tile(uint32_t *ticket, uint32_t count, uint32_t *
   return *flag != 0;
 }
 
+// Which tile and range of keys a workgroup of the kernel for few rows takes, and where the tile's partial results and its
+// ticket lie.
+struct RangePlace {
+  Place at;
+  uint32_t range;
+  uint32_t part, step;  // partial result of the tile's first range, and how far the next is behind it
+  uint32_t ticket;
+};
+
+// listed == 0: every tile has `splits` ranges, of which a short sequence leaves most without work.  Otherwise entry i of the
+// list, with k_cum keys before it, owns the slots from floor(k_cum / chunk) + i on, which is room for its ranges (as in
+// find_place for tiles), and a slot has `tiles` tiles; behind the slots come the tiles of tokens of no sequence.
+template <typename T>
+__device__ inline RangePlace find_range(const FwArgs<T> &a, uint32_t index, uint32_t head, int lane) {
+  const Shape &sh = a.s;
+  if (a.listed == 0) {
+    const uint32_t slot = index / a.splits, tile = slot * sh.hk + head;
+    return {find_place(a.seq, slot, a.tiles, 32, sh.g, false, sh.causal != 0), index - slot * a.splits, tile * a.splits, 1, tile};
+  }
+  const uint32_t slot = index / a.tiles, t = index - slot * a.tiles;
+  if (slot >= a.listed)
+    return {{{kNoSequence, 0, 0, 0, 0, 0, 0, 0}, uniform(index - a.listed * a.tiles)}, 0, 0, 0, 0};
+  // the last entry whose first slot is not behind `slot`: 64 candidates at a time, one per lane
+  uint32_t lo = 0, count = a.seq.n;
+  while (count > 1) {
+    const uint32_t stride = (count + 63) / 64, i = lo + (uint32_t)lane * stride;
+    const bool mine = (uint32_t)lane * stride < count && a.seq.entries[i].k_cum / a.chunk + i <= slot;
+    const uint32_t found = (uint32_t)__popcll(__ballot(mine)) - 1;  // lane 0's is true
+    lo += found * stride;
+    count = min(stride, count - found * stride);
+  }
+  lo = uniform(lo);
+  const SequenceEntry e = uniform(a.seq.entries[lo]);
+  const uint32_t first = e.k_cum / a.chunk + lo;
+  const uint32_t own = a.seq.packed ? (uint32_t)(((uint64_t)e.q_len * sh.g + 31) / 32) : a.tiles;
+  return {{e, uniform(sh.causal && t < own ? own - 1 - t : t)}, slot - first, (first * a.tiles + t) * sh.hk + head,
+          a.tiles * sh.hk, (lo * a.tiles + t) * sh.hk + head};
+}
+
 template <typename T, int DP, bool DMA, int W>
 __global__ __launch_bounds__(64 * W, 1) void few_kernel(const FwArgs<T> a) {
   constexpr int BM = 32, S = kStages<T, DP>, kThreads = 64 * W;
@@ -333,8 +375,10 @@ __global__ __launch_bounds__(64 * W, 1) void few_kernel(const FwArgs<T> a) {
 
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const Shape &sh = a.s;
-  const uint32_t head = blockIdx.x % sh.hk, range = blockIdx.x / sh.hk % a.splits, slot = blockIdx.x / sh.hk / a.splits;
-  const Place at = find_place(a.seq, slot, a.tiles, BM, sh.g, false, sh.causal != 0);
+  const uint32_t head = blockIdx.x % sh.hk;
+  const RangePlace place = find_range(a, blockIdx.x / sh.hk, head, lane);
+  const Place &at = place.at;
+  const uint32_t range = place.range;
   const SequenceEntry &e = at.e;
   const bool behind = e.sample == kNoSequence;
   const uint32_t token0 = behind ? a.seq.q_total : e.q_start;
@@ -359,7 +403,7 @@ __global__ __launch_bounds__(64 * W, 1) void few_kernel(const FwArgs<T> a) {
   Frag<T> qf[DP / 16];
   {
     const size_t row = row_base + walk.at(exists ? lane & 31 : 0, sh.hq);
-  load_row<T>(qf, a.q + row * sh.d, valid, sh, lane);
+    load_row<T>(qf, a.q + row * sh.d, valid, sh, lane);
   }
   Rows<DP> st;
   reset(st);
@@ -450,8 +494,8 @@ __global__ __launch_bounds__(64 * W, 1) void few_kernel(const FwArgs<T> a) {
   }
   __syncthreads();
   const bool whole = ranges == 1;
-  const uint32_t tile = slot * sh.hk + head;
-  float *const part = a.partial + ((size_t)tile * a.splits + range) * (size_t)(BM * (DP + 4));
+  const size_t part_size = (size_t)a.part_rows * (DP + 4);
+  float *const all_parts = a.partial + place.part * part_size, *const part = all_parts + (size_t)range * place.step * part_size;
   // four elements of a row
   auto finish = [&](int row, uint32_t dd, const float (&o)[4], float m, float l) {
     const size_t at_row = row_base + walk.at((uint32_t)row, sh.hq);
@@ -490,10 +534,9 @@ __global__ __launch_bounds__(64 * W, 1) void few_kernel(const FwArgs<T> a) {
       }
     }
   }
-  if (whole || !last_of_tile(a.tickets + tile, ranges, &flag)) return;
+  if (whole || !last_of_tile(a.tickets + place.ticket, ranges, &flag)) return;
   // The last of the tile: each thread has an element of a row at a time and takes the ranges 16 at a time, all their
   // loads in flight together.
-  const float *const all_parts = a.partial + (size_t)tile * a.splits * (size_t)(BM * (DP + 4));
   for (uint32_t i = tid; i < (uint32_t)rows * DP; i += kThreads) {
     const int row = (int)(i / DP);
     const uint32_t dd = i % DP;
@@ -502,7 +545,7 @@ __global__ __launch_bounds__(64 * W, 1) void few_kernel(const FwArgs<T> a) {
       float pm[16], pl[16], po[16];
 #pragma unroll
       for (uint32_t u = 0; u < 16; ++u) {
-        const float *p = all_parts + (size_t)min(p0 + u, ranges - 1) * (BM * (DP + 4)) + row * (DP + 4);
+        const float *p = all_parts + (size_t)min(p0 + u, ranges - 1) * place.step * part_size + row * (DP + 4);
         pm[u] = load_shared(p + DP);
         pl[u] = load_shared(p + DP + 1);
         po[u] = load_shared(p + dd);
@@ -567,19 +610,36 @@ int launch_few(phip_ctx *ctx, FwArgs<T> a, const phip_sequences *seqs) {
   const uint32_t most = seqs != nullptr ? seqs->max_k : a.seq.tk;
   a.chunk = W == 1 ? most + 1 : few_chunk(ctx, a.seq, seqs, tiles);
   a.splits = most <= a.chunk ? 1 : (most + a.chunk - 1) / a.chunk;
-  PHIP_REQUIRE(launchable(tiles * a.splits, 64 * W), "too many rows");
+  uint64_t blocks = tiles * a.splits, parts = blocks;
+  const uint64_t most_rows = std::max<uint64_t>(1, (uint64_t)(a.seq.packed ? seqs->max_q : a.seq.tq) * a.s.g);
+  a.part_rows = (uint32_t)std::min<uint64_t>(32, most_rows);
+  if (a.splits > 1 && seqs != nullptr && seqs->k_sum <= 0xffffffffu) {
+    // One long sequence among many short ones: its ranges times all tiles would be mostly empty workgroups, each with a place
+    // in the scratch memory (131072 keys beside 127 times 64, one key head: 512 MB and 137 us; listed 4 MB and 62 us).  With
+    // fewer than four places per range that exists the plain order is the faster one (31 streams of 1 to 8192 keys, 8 key
+    // heads, 2.5 places: 67 us, listed 80).
+    const uint64_t per = (most_rows + 31) / 32, listed = seqs->k_sum / a.chunk + a.seq.n, own = listed * per * a.s.hk;
+    const uint64_t behind = a.seq.packed ? ((uint64_t)(a.seq.tq - a.seq.q_total) * a.s.g + 31) / 32 * a.s.hk : 0;
+    if (4 * (own + behind) <= blocks && a.seq.n * per * a.s.hk <= (uint64_t)kTicketSlots) {
+      a.listed = (uint32_t)listed;
+      a.tiles = (uint32_t)per;
+      blocks = own + behind;
+      parts = own;
+    }
+  }
+  PHIP_REQUIRE(launchable(blocks, 64 * W), "too many rows");
   void *partial = nullptr;
   if (a.splits > 1) {
-    const int rc2 = phip_pool_alloc(ctx, (size_t)tiles * a.splits * 32 * (DP + 4) * sizeof(float), &partial, nullptr);
+    const int rc2 = phip_pool_alloc(ctx, (size_t)parts * a.part_rows * (DP + 4) * sizeof(float), &partial, nullptr);
     if (rc2 != PHIP_OK) return rc2;
     a.partial = static_cast<float *>(partial);
     a.tickets = tile_tickets(ctx);
   }
-  hipLaunchKernelGGL((few_kernel<T, DP, DMA, W>), dim3((uint32_t)(tiles * a.splits)), dim3(64 * W), lds, ctx->stream, a);
+  hipLaunchKernelGGL((few_kernel<T, DP, DMA, W>), dim3((uint32_t)blocks), dim3(64 * W), lds, ctx->stream, a);
   const hipError_t e = hipGetLastError();
   if (partial != nullptr) phip_pool_free(ctx, partial);
   if (e != hipSuccess) return fail(PHIP_ERR_RUNTIME, "launching the attention kernel failed: %s", hipGetErrorString(e));
-  note_kernel(ctx, W == 1 ? "attention_few1" : a.splits > 1 ? "attention_few_split" : "attention_few");
+  note_kernel(ctx, W == 1 ? "attention_few1" : a.listed ? "attention_few_listed" : a.splits > 1 ? "attention_few_split" : "attention_few");
   return PHIP_OK;
 }
 

@@ -8,7 +8,7 @@ namespace phip {
 
 // One sequence, as the attention kernels read it.  The entries are sorted by falling length (keys, then queries), so
 // that the tiles of the longest sequences are launched first; q_cum and k_cum count the tokens of the entries before
-// this one in that order.
+// this one in that order (modulo 2^32; read only where the totals fit).
 struct SequenceEntry {
   uint32_t sample;            // padded: which sample; packed: 0
   uint32_t q_start, q_len;    // first token (packed only, else 0) and number of tokens

@@ -51,7 +51,7 @@ int create(phip_ctx *ctx, const uint32_t *q_lens, const uint32_t *k_lens, uint32
   std::stable_sort(entries.begin(), entries.end(), [](const SequenceEntry &a, const SequenceEntry &b) {
     return a.k_len != b.k_len ? a.k_len > b.k_len : a.q_len > b.q_len;
   });
-  uint32_t q_cum = 0, k_cum = 0;  // used for packed sequences only, whose totals fit
+  uint32_t q_cum = 0, k_cum = 0;  // read only where the totals fit
   for (SequenceEntry &e : entries) {
     e.q_cum = q_cum;
     e.k_cum = k_cum;

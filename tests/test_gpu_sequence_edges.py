@@ -424,3 +424,65 @@ def test_attention_of_very_many_fp32_sequences():
         assert (t.to_vector() == want).all()
     del q, k, v, y, stats, g
     dev.close()
+
+
+# Lists of which one sequence is much longer than the others: workgroups only for ranges of keys that exist
+LISTED = {
+    "packed_one_long": (128, 8, 1, 140, 28200, 1, (1,) * 128, (64,) * 100 + (20000,) + (64,) * 27, True, True),
+    "packed_some_empty": (64, 8, 2, 40, 9000, 1, (1, 0, 3, 1, 0, 2, 1) * 4, (10, 4000, 3, 0, 0, 400, 1000) + (10, 300, 3, 0, 0, 400, 100) * 3, True, True),
+    "packed_not_causal": (33, 2, 2, 30, 8000, 1, (1, 2) * 10, (7000, 1) + (1, 7) * 9, True, False),
+    "padded_one_long": (64, 8, 2, 1, 7000, 20, (1,) * 20, (7, 7000, 0, 300, 64) + (100,) * 15, False, True),
+    "padded_five_tokens": (128, 16, 2, 5, 5000, 12, (5, 0, 3) * 4, (5000, 9, 1) + (5, 600, 2) * 3, False, True),
+    "padded_odd_size": (65, 6, 2, 2, 4000, 9, (2, 1, 2) * 3, (30, 4000, 700) + (2, 1, 0) * 2, False, False),
+}
+
+
+@pytest.mark.parametrize("name", sorted(LISTED))
+@pytest.mark.parametrize("kind", KINDS)
+def test_attention_of_one_long_sequence_among_short_ones(devices, kind, name):  # noqa: F811
+    dev = devices[kind]
+    d, hq, hk, tq, tk, bs, q_lens, k_lens, packed, causal = LISTED[name]
+    rng = np.random.default_rng(80 + len(name))
+    q, k, v = (draw(rng, kind, bs, t, h, d) for t, h in ((tq, hq), (tk, hk), (tk, hk)))
+    seqs = places(bs, tq, tk, q_lens, k_lens, packed)
+    scale = 1.0 / float(np.sqrt(d))
+    want = Attention(q, k, v, seqs, causal, scale, kind)
+    used_q, used_k = np.zeros(q.shape[:2], bool), np.zeros(k.shape[:2], bool)
+    for b, aq, n, ak, m in seqs:
+        used_q[b, aq:aq + n] = used_k[b, ak:ak + m] = True
+    q[~used_q], k[~used_k], v[~used_k] = np.nan, np.nan, np.inf
+    t = [tensor(dev, x) for x in (q, k, v)]
+    lists = dev.new_sequences(q_lens, k_lens, packed)
+    seen = []
+    for _ in range(3):   # the tickets are left as they were found
+        dev.gemm_trace(True)
+        y, stats = dev.attention_fw(*t, causal, scale, lists, stats=True)
+        assert dev.gemm_trace(False) == ["attention_few_listed"]
+        seen.append(y.to_vector())
+        check("y", seen[-1], want.y, want.tol_y)
+        got = stats.to_vector().reshape(want.stats.shape)
+        assert np.array_equal(np.isneginf(got), np.isneginf(want.stats))
+        some = ~np.isneginf(want.stats)
+        check("stats", got[some], want.stats[some], want.tol_stats[some])
+    assert np.array_equal(seen[0], seen[1]) and np.array_equal(seen[0], seen[2])
+
+
+def test_memory_of_one_long_sequence_among_short_ones():
+    """Partial results for the ranges that exist: some 10 MB, not for the longest's ranges of every sequence."""
+    dev = pa.HIP16(0, storage="bf16")
+    hip = ctypes.CDLL("libamdhip64.so")
+    free, total = ctypes.c_size_t(), ctypes.c_size_t()
+
+    def left():
+        _lib.call("phip_sync", dev.ctx())
+        assert hip.hipMemGetInfo(ctypes.byref(free), ctypes.byref(total)) == 0
+        return free.value
+    lens = [131072] + [64] * 127
+    q, k = dev.new_tensor_by_constant(S([128, 8, len(lens)]), 1), dev.new_tensor_by_constant(S([128, 1, sum(lens)]), 1)
+    lists, y = dev.new_sequences([1] * len(lens), lens, True), dev.attention_fw(q, k, k)
+    before = left()
+    y = dev.attention_fw(q, k, k, True, None, lists)
+    assert before - left() < 64 << 20
+    assert (y.to_vector() == 1).all()
+    del q, k, y, lists
+    dev.close()
