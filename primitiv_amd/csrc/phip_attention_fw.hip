@@ -589,15 +589,18 @@ int launch_rows(phip_ctx *ctx, FwArgs<T> a) {
 }
 
 // Keys per range of the kernel for few rows.  One workgroup of four wavefronts fits on a CU (its ring of tiles), so the
-// time is about the keys of a range times the rounds that the ranges take on the chip: ranges that fill it about once.
+// time is about the keys of a range times the rounds that the ranges take on the chip: a range is a CU's share of all keys,
+// and where the longest sequence is less than two shares it is left whole, because its second range would wait for a CU.
+// One token each, 32/8 heads of 128, bf16, us whole -> cut: 17 streams of 4096 keys (1.9 shares) 50 -> 64, 31 of them (1.03)
+// 51 -> 102, 32 streams of 1 to 8192 (1.8) 92 -> 117; four of 8192 beside 60 of 1000 (2.8) 90 -> 58, one of 8192 beside 31 of
+// 512 (11) 89 -> 25.
 uint32_t few_chunk(phip_ctx *ctx, const SequenceView &view, const phip_sequences *seqs, uint64_t tiles) {
   const uint64_t cus = (uint64_t)ctx->prop.multiProcessorCount;
   const uint64_t most = seqs != nullptr ? seqs->max_k : view.tk;
-  if (tiles >= cus || tiles > (uint64_t)kTicketSlots) return (uint32_t)most + 1;
   const uint64_t sum = seqs != nullptr ? seqs->k_sum : (uint64_t)view.n * view.tk;
-  uint64_t chunk = sum * tiles / view.n / cus;
-  if (chunk < 256) chunk = 256;
-  return (uint32_t)std::min<uint64_t>((chunk + 127) / 128 * 128, 1u << 30);
+  const uint64_t share = sum * tiles / view.n / cus;
+  if (most < 2 * share || tiles > (uint64_t)kTicketSlots) return (uint32_t)most + 1;
+  return (uint32_t)std::min<uint64_t>((std::max<uint64_t>(share, 256) + 127) / 128 * 128, 1u << 30);
 }
 
 template <typename T, int DP, bool DMA, int W>

@@ -486,3 +486,22 @@ def test_memory_of_one_long_sequence_among_short_ones():
     assert (y.to_vector() == 1).all()
     del q, k, y, lists
     dev.close()
+
+
+@pytest.mark.parametrize("lens,kernel", (
+    ((4096,) * 16, "attention_few_split"), ((4096,) * 17, "attention_few"), ((4096,) * 31, "attention_few"),
+    ((4096,) * 40, "attention_few"), ((8192,) + (512,) * 30, "attention_few_listed"), ((8192,) + (512,) * 31, "attention_few_listed"),
+    ((8192,) + (512,) * 63, "attention_few_listed"), ((8192,) * 4 + (1000,) * 60, "attention_few_split")))
+def test_keys_are_cut_by_the_lengths_not_by_the_number_of_streams(lens, kernel):
+    dev = pa.HIP16(0, storage="bf16")
+    n = len(lens)
+    q, k = dev.new_tensor_by_constant(S([128, 32, 1], n), 1), dev.new_tensor_by_constant(S([128, 8, max(lens)], n), 1)
+    lists = dev.new_sequences((1,) * n, lens)
+    dev.gemm_trace(True)
+    y, stats = dev.attention_fw(q, k, k, True, 0.01, lists, stats=True)
+    assert dev.gemm_trace(False) == [kernel]
+    assert (y.to_vector() == 1).all()
+    # scores of 1.28: fp32 sums of up to 8192 equal terms
+    check("stats", stats.to_vector().reshape(n, 32), np.repeat(1.28 + np.log(np.float64(lens))[:, None], 32, 1), 1e-4)
+    del q, k, y, stats, lists
+    dev.close()
