@@ -542,14 +542,23 @@ constexpr int kStages = 32 * Tile<T, DP>::kPitch <= 8192 ? 2 : 1;
 // fp32 products take four times as long per tile, which hides the loads of the finer division: there it also wins with a
 // workgroup per CU when the walk is long (16 heads of 65, 1 x 2048: 1068 -> 740).
 // One wavefront per workgroup: fp32 sequences so short that a 128-row tile is mostly empty and so many that every SIMD has
-// one anyway (16 heads of 65, 64 x 35 tokens: 217 -> 157; in 16-bit storage it does not pay: 125 against 157).
+// one anyway (in 16-bit storage it does not pay: 16 heads of 65, 64 x 35 tokens: 125 against 157).  us per training step
+// without -> with, by the number of 32-row tiles:
+//                                512            1024           4096
+//   8 tokens, 8 heads of 128     80 -> 44       154 -> 50      619 -> 185
+//   32 tokens, 16 of 64          50 -> 32       98 -> 43       370 -> 164
+//   35 tokens, 10 of 65          66 -> 71       116 -> 87      441 -> 295
+//   64 tokens, 16 of 64          40 -> 43       69 -> 52       240 -> 196  (forward alone 43 -> 51)
+//   96 tokens, 16 of 64          52 -> 54       92 -> 62       253 -> 221
+//   128 tokens, 16 of 64         64 -> 65       70 -> 73       233 -> 250
+// Walks of more than 256 keys (rows) want the 1024 tiles too: 4 queries, 500 keys, 8 heads of 128, forward: 58 -> 84 and 117 -> 96.
 enum class Way { Shared, Four, One };
 // wide, narrow: workgroups with tiles of 128 and of 32; most: rows (keys) of the longest sequence; walked: what its
 // workgroups walk over.
 template <typename T>
 inline Way choose_way(phip_ctx *ctx, uint64_t wide, uint64_t narrow, uint64_t most, uint64_t walked) {
   const uint64_t cus = (uint64_t)ctx->prop.multiProcessorCount;
-  if (sizeof(T) == 4 && most <= 64 && narrow >= 2 * cus) return Way::One;
+  if (sizeof(T) == 4 && most <= 64 && narrow >= (most <= 32 && walked <= 256 ? 2 : 4) * cus) return Way::One;
   if (wide * 2 <= cus || (sizeof(T) == 4 && wide <= cus && walked >= 1024)) return Way::Four;
   return Way::Shared;
 }

@@ -149,7 +149,7 @@ SHORT = {
     "whole": (64, 16, 16, 35, 35, 33, None, None, False, True),
     "odd_size": (65, 10, 10, 35, 35, 64, None, None, False, True),
     "size_1": (1, 16, 16, 50, 50, 33, None, None, False, False),
-    "size_33": (33, 16, 16, 64, 64, 17, None, None, False, True),
+    "size_33": (33, 16, 16, 64, 64, 33, None, None, False, True),
     "grouped": (128, 32, 16, 20, 31, 40, None, None, False, True),
     "padded": (96, 16, 16, 60, 64, 36, (60, 0, 1, 33) * 9, (60, 9, 3, 64) * 9, False, True),
     "packed": (80, 40, 40, 400, 430, 1, (33, 1, 0, 60, 17) * 3, (35, 1, 9, 64, 0) * 3, True, True),
@@ -505,3 +505,16 @@ def test_keys_are_cut_by_the_lengths_not_by_the_number_of_streams(lens, kernel):
     check("stats", stats.to_vector().reshape(n, 32), np.repeat(1.28 + np.log(np.float64(lens))[:, None], 32, 1), 1e-4)
     del q, k, y, stats, lists
     dev.close()
+
+
+@pytest.mark.parametrize("tokens,keys,batch,one", ((8, 8, 64, True), (8, 8, 63, False), (32, 256, 64, True), (32, 257, 64, False),
+                                                   (35, 35, 64, True), (35, 35, 63, False), (65, 65, 128, False)))
+def test_which_fp32_sequences_take_a_wavefront_each(devices, tokens, keys, batch, one):  # noqa: F811
+    """From 512 tiles of 32 rows on, or from 1024 on where they are two to a sequence or walk far."""
+    dev = devices["f32"]
+    q, k = (dev.new_tensor_by_constant(S([16, 8, t], batch), 1) for t in (tokens, keys))
+    dev.gemm_trace(True)
+    y = dev.attention_fw(q, k, k)
+    assert (dev.gemm_trace(False) == ["attention_few1"]) == one
+    # the weights and the weighted ones are added up apart (half a step a term), then divided
+    assert np.abs(y.to_vector() - 1).max() <= (2 * keys + 2) * 2.0 ** -24
