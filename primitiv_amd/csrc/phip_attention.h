@@ -96,7 +96,8 @@ __device__ inline uint32_t round_pair(float x0, float x1) {
 }
 
 // Registers 8 c .. 8 c + 7 of a block as the right operand of the next product.  16-bit storage rounds here: the matrix
-// instruction takes no wider operand, and the probabilities carry one rounding as a stored probability matrix would.
+// instruction takes no wider operand, and the probabilities carry one rounding as a stored probability matrix would (the
+// kernel for few rows adds what the rounding leaves out; dS is rounded once, too).
 // fp16 rounds to a fixed step below 2^-14, and the thousands of probabilities that add up to a result may all lie there: they
 // are kept kRaise powers of two higher (2^14 for a probability of 1, of the 2^16 that fp16 holds), so that only those below
 // 2^-28 of the largest lose bits.  It costs nothing forward: the raise is part of the exponent, and the sum carries it too.

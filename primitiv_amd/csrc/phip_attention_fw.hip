@@ -27,6 +27,7 @@ struct FwArgs {
   uint32_t chunk;
   uint32_t splits;      // ranges of the longest sequence; a workgroup for each range of each tile, or,
   uint32_t listed;      // if not 0: workgroups for the ranges that the listed sequences have (see find_range): their slots
+  uint32_t exact;       // probabilities in two parts
   uint32_t part_rows;   // rows of a tile that exist at most
   float *partial;       // per tile and range: part_rows x (DP sums, maximum, sum, 2 unused)
   uint32_t *tickets;
@@ -159,9 +160,23 @@ __device__ inline bool values_masked(Rows<DP> &st, const Scores<KB> &sc, uint32_
   return true;
 }
 
-// The product with the values.
+// What the rounding of an operand left out, rounded in turn.
+template <typename T>
+__device__ inline Frag16<T> left_out(const f32x16 &p, int c, const Frag16<T> &f) {
+  Frag16<T> r;
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+    r.v[e] = round_pair<T>(p[8 * c + 2 * e] - element(f, 2 * e), p[8 * c + 2 * e + 1] - element(f, 2 * e + 1));
+  return r;
+}
+
+// The product with the values.  exact (16-bit storage): the probabilities in two parts, which together carry 16 bits (bf16) or
+// 22 (fp16).  Taken where a sequence's rows are one tile, the single tokens of a serving loop: those calls wait for memory, so
+// the second product costs 1 to 5 % (one token of 31 streams of 4096 keys, 32/8 heads of 128, bf16: 95 -> 96 us; 130001 keys,
+// fp16: 105 -> 106) and the result is as far from the exact one as its own rounding (root mean square error 1.27 and 1.33 ->
+// 1.0 times that).  Prompts are bound by the products and the vector instructions and take one part.
 template <typename T, int DP, int KB>
-__device__ inline void values(Rows<DP> &st, const Scores<KB> &sc, uint32_t v_at) {
+__device__ inline void values(Rows<DP> &st, const Scores<KB> &sc, uint32_t v_at, bool exact) {
 #pragma unroll
   for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
@@ -169,6 +184,13 @@ __device__ inline void values(Rows<DP> &st, const Scores<KB> &sc, uint32_t v_at)
       const Frag<T> p = as_operand(sc.s[kb], c, (Frag<T> *)nullptr);
 #pragma unroll
       for (int db = 0; db < DP / 32; ++db) mma(st.o[db], Tile<T, DP>::col_frag(v_at, 2 * kb + c, db), p);
+      if constexpr (sizeof(T) == 2) {
+        if (exact) {
+          const Frag<T> rest = left_out<T>(sc.s[kb], c, p);
+#pragma unroll
+          for (int db = 0; db < DP / 32; ++db) mma(st.o[db], Tile<T, DP>::col_frag(v_at, 2 * kb + c, db), rest);
+        }
+      }
     }
 }
 
@@ -278,7 +300,7 @@ __global__ __launch_bounds__(kThreads, 2) void rows_kernel(const FwArgs<T> a) {
       softmax<T, DP, KT / 32>(st, sc, t * KT, lim, (t + 1) * KT > w_all, sh.scale_log2, lane);
       const bool masked = (t + 1) * KT > w_all;
       if (!masked || !values_masked<T, DP, KT / 32>(st, sc, stage + kTile + col_at, t * KT, lim, lane))
-        values<T, DP, KT / 32>(st, sc, stage + kTile + col_at);
+        values<T, DP, KT / 32>(st, sc, stage + kTile + col_at, false);
     }
   }
 
@@ -443,7 +465,7 @@ __global__ __launch_bounds__(64 * W, 1) void few_kernel(const FwArgs<T> a) {
       softmax<T, DP, 1>(st, sc, key, lim, key + 32 > all, sh.scale_log2, lane);
       wait_loads<kInFlight>();
       if (key + 32 <= first_sees || !values_masked<T, DP, 1>(st, sc, stage + kTile + col_at, key, lim, lane))
-        values<T, DP, 1>(st, sc, stage + kTile + col_at);
+        values<T, DP, 1>(st, sc, stage + kTile + col_at, a.exact != 0);
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
       fetch_v(key + S * kStep, s);
     }
@@ -464,7 +486,7 @@ __global__ __launch_bounds__(64 * W, 1) void few_kernel(const FwArgs<T> a) {
       scores<T, DP, 1>(sc, qf, ring + row_at);
       softmax<T, DP, 1>(st, sc, key, lim, key + 32 > all, sh.scale_log2, lane);
       if (key + 32 <= first_sees || !values_masked<T, DP, 1>(st, sc, ring + kTile + col_at, key, lim, lane))
-        values<T, DP, 1>(st, sc, ring + kTile + col_at);
+        values<T, DP, 1>(st, sc, ring + kTile + col_at, a.exact != 0);
     }
   }
 
@@ -616,6 +638,7 @@ int launch_few(phip_ctx *ctx, FwArgs<T> a, const phip_sequences *seqs) {
   uint64_t blocks = tiles * a.splits, parts = blocks;
   const uint64_t most_rows = std::max<uint64_t>(1, (uint64_t)(a.seq.packed ? seqs->max_q : a.seq.tq) * a.s.g);
   a.part_rows = (uint32_t)std::min<uint64_t>(32, most_rows);
+  a.exact = sizeof(T) == 2 && most_rows <= 32 ? 1 : 0;
   if (a.splits > 1 && seqs != nullptr && seqs->k_sum <= 0xffffffffu) {
     // One long sequence among many short ones: its ranges times all tiles would be mostly empty workgroups, each with a place
     // in the scratch memory (131072 keys beside 127 times 64, one key head: 512 MB and 137 us; listed 4 MB and 62 us).  With

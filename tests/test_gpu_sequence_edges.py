@@ -518,3 +518,18 @@ def test_which_fp32_sequences_take_a_wavefront_each(devices, tokens, keys, batch
     assert (dev.gemm_trace(False) == ["attention_few1"]) == one
     # the weights and the weighted ones are added up apart (half a step a term), then divided
     assert np.abs(y.to_vector() - 1).max() <= (2 * keys + 2) * 2.0 ** -24
+
+
+@pytest.mark.parametrize("kind", KINDS[1:])
+@pytest.mark.parametrize("shape", ((1, 300, 64, 8, 2, 3), (4, 2000, 128, 16, 4, 1), (1, 700, 65, 3, 3, 2)))
+def test_single_tokens_in_16_bits_lose_nothing_but_the_results_rounding(devices, kind, shape):  # noqa: F811
+    """Where a sequence's rows are one tile, the probabilities keep twice the storage type's bits."""
+    dev, h = devices[kind], HALF[kind]
+    tq, tk, d, hq, hk, bs = shape
+    rng = np.random.default_rng(90 + tk)
+    q, k, v = (draw(rng, kind, bs, t, n, d) for t, n in ((tq, hq), (tk, hk), (tk, hk)))
+    args = (places(bs, tq, tk), True, 0.125, kind)
+    want, size = Attention(q, k, v, *args), Attention(q, k, np.abs(v), *args).y   # size: the sum of |P v|
+    y = dev.attention_fw(*(tensor(dev, x) for x in (q, k, v)), True, 0.125)
+    # the bound allows one rounding (h) of each probability: what is left of it is the rounding of the second part, h h
+    check("y", y.to_vector(), want.y, want.tol_y - 1.05 * (h - h * h) * size)
