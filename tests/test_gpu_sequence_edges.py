@@ -533,3 +533,19 @@ def test_single_tokens_in_16_bits_lose_nothing_but_the_results_rounding(devices,
     y = dev.attention_fw(*(tensor(dev, x) for x in (q, k, v)), True, 0.125)
     # the bound allows one rounding (h) of each probability: what is left of it is the rounding of the second part, h h
     check("y", y.to_vector(), want.y, want.tol_y - 1.05 * (h - h * h) * size)
+
+
+# Groups larger than a tile of rows, up to the largest: (heads, batch, kernels of bf16)
+@pytest.mark.parametrize("kind,heads,batch,kernels", (
+    ("f32", 1024, 1, ("attention_few", "attention_few_queries", "attention_few_keys")),
+    ("f16", 300, 1, ("attention_few", "attention_few_queries", "attention_few_keys")),
+    ("bf16", 1024, 6, ("attention_rows", "attention_queries", "attention_few_keys"))))
+def test_attention_of_large_groups(devices, kind, heads, batch, kernels):  # noqa: F811
+    attention_against_reference(devices[kind], kind, (16, heads, 1, 3, 40, batch, None, None, False, True), 100, kernels)
+
+
+def test_a_larger_group_is_refused(devices):  # noqa: F811
+    dev = devices["f32"]
+    q, k = (dev.new_tensor_by_constant(S([16, h, 2]), 1) for h in (1025, 1))
+    with pytest.raises(pa.Error, match="1024 query heads"):
+        dev.attention_fw(q, k, k)
