@@ -59,10 +59,10 @@ __device__ inline float row_base(float stats) { return stats == -INFINITY ? INFI
 
 // dS in fp16.  It is a probability, of thousands of keys perhaps, times a difference of any size: 2^-40 and 2^20 are ordinary
 // values, and fp16 has neither.  So a wavefront scales its dS by a power of two before it is rounded, and its sums with it:
-// the first block puts the largest between 2^9 and 2^13, and a block that exceeds 2^15 scales everything down to that again.
-// What is below 2^-23 of the largest so far loses bits; nothing overflows.  Eight maxima and a multiplication per 16 values
-// (queries: part of the multiply-add), the rest is rare: a training step with heads of 64 takes 3 to 4 % longer than with dS
-// rounded as it is (16 heads, 8192 tokens: 815 against 784 us), with heads of 128 no longer.
+// the first block puts the largest between 2^13 and 2^14, and a block that goes beyond fp16 scales everything down to that
+// again.  What is below 2^-27 of the largest so far loses bits; nothing overflows.  Eight maxima and a multiplication per 16
+// values (queries: part of the multiply-add), the rest is rare: a training step with heads of 64 takes 3 to 4 % longer than
+// with dS rounded as it is (16 heads, 8192 tokens: 860 against 832 us), with heads of 128 no longer.
 template <typename T>
 constexpr bool kRanged = __is_same(T, f16_t);
 struct Range {
@@ -73,14 +73,18 @@ struct Range {
 // m: the largest |x| of the lane's 16 values.  Returns what x and the sums were multiplied by.
 template <int N>
 __device__ inline float fit(Range &range, f32x16 &x, f32x16 (&sums)[N], float m) {
-  if (range.known && !__any(m > 0x1p15f)) return 1.f;
+  if (range.known && !__any(m > 0x1.ffp15f)) return 1.f;
   if (!__any(m > 0.f)) return 1.f;
   float by = 1.f;
-  // steps of 16, as many as the range of a float has: infinite values stay what they are
+  // In steps of 16 to between 2^14 and 2^18, then down in steps of 2.  Up by 2^64 at most: what follows may be as large as fp16
+  // operands allow (a raised probability of 2^15 times two sums of 128 products of 2^32: 2^55) and must not exceed fp32 before
+  // it is seen here; if nothing larger follows, the gradients are below fp16 anyway.  Infinite values stay what they are.
 #pragma unroll 1
-  for (int i = 0; i < 24 && !__any(m * by >= 0x1p9f); ++i) by *= 0x1p4f;
+  for (int i = 0; i < 16 && !__any(m * by >= 0x1p14f); ++i) by *= 0x1p4f;
 #pragma unroll 1
-  for (int i = 0; i < 24 && __any(m * by > 0x1p13f); ++i) by *= 0x1p-4f;
+  for (int i = 0; i < 32 && __any(m * by >= 0x1p18f); ++i) by *= 0x1p-4f;
+#pragma unroll 1
+  for (int i = 0; i < 4 && __any(m * by >= 0x1p14f); ++i) by *= 0.5f;
   range.known = true;
   range.scale *= by;
 #pragma unroll

@@ -549,3 +549,26 @@ def test_a_larger_group_is_refused(devices):  # noqa: F811
     q, k = (dev.new_tensor_by_constant(S([16, h, 2]), 1) for h in (1025, 1))
     with pytest.raises(pa.Error, match="1024 query heads"):
         dev.attention_fw(q, k, k)
+
+
+@pytest.mark.parametrize("shape", ((128, 33, 1, 7, 400, 1, None, None, False, True), (64, 10, 2, 200, 1500, 1, None, None, False, True),
+                                   (64, 8, 8, 70, 300, 35, None, None, False, True)))
+@pytest.mark.parametrize("size", (1.0, 300.0))
+def test_fp16_gradients_with_scores_of_hundreds(devices, shape, size):  # noqa: F811
+    """Probabilities from 2^-140 to 1 in one row: the first block of keys may have hardly any weight, the next nearly all."""
+    dev = devices["f16"]
+    d, hq, hk, tq, tk, bs = shape[:6]
+    rng = np.random.default_rng(0)
+    q, k, v, gy = (rounded(rng.standard_normal((bs, t, h, d)) * f, "f16") for t, h, f in (
+        (tq, hq, 6), (tk, hk, 6), (tk, hk, 1), (tq, hq, size)))
+    want = Attention(q, k, v, places(bs, tq, tk), True, 1.0, "f16", gy)
+    t = [tensor(dev, x) for x in (q, k, v, gy)]
+    y, stats = dev.attention_fw(*t[:3], True, 1.0, None, stats=True)
+    g = [dev.new_tensor_by_constant(x.shape(), 0) for x in t[:3]]
+    dev.attention_bw(*t[:3], y, t[3], stats, True, 1.0, None, *g)
+    # dS is rounded to half of a step of 2^-24 where its largest is 2^13 or more: 2^-38 of the largest, at most 2 d |gy| |v|
+    step = 2.0 ** -38 * 2 * d * np.abs(gy).max() * np.abs(v).max() * max(np.abs(q).max(), np.abs(k).max()) * max(tk, tq * hq // hk)
+    for x, n in zip((y, *g), ("y", "gq", "gk", "gv")):
+        r = getattr(want, n)
+        assert np.abs(r).max() < 65504
+        check(n, x.to_vector(), r, getattr(want, "tol_" + n) + (step if n in ("gq", "gk") else 0))
