@@ -669,8 +669,8 @@ int phip_sequences_destroy(phip_sequences *seqs);
  * No counterpart in the reference.  Rotates the first 2*pairs elements of each
  * head of the queries xq ([d, hq, t] x bs) and of the keys xk ([d, hk, t] x bs;
  * NULL with hk == 0: queries only) of the same tokens, pair i by the angle
- * position * freqs[i] (the product is exact: far positions lose nothing), and
- * copies the rest of the head.  Pair i is (x[i], x[i + pairs]), or with
+ * position * freqs[i] (in 64 bits: far positions lose nothing), and copies the
+ * rest of the head.  Pair i is (x[i], x[i + pairs]), or with
  * interleaved != 0 (x[2i], x[2i+1]); the rotated elements are scaled by
  * `amplitude` (1 for plain rotation).  freqs: HOST array of `pairs` values.  The
  * position of a token is first + its position in its sequence (`seqs`; NULL:

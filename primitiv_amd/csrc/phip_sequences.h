@@ -12,7 +12,7 @@ namespace phip {
 struct SequenceEntry {
   uint32_t sample;            // padded: which sample; packed: 0
   uint32_t q_start, q_len;    // first token (packed only, else 0) and number of tokens
-  uint32_t k_start, k_len;
+  uint32_t k_start, k_len;    // (k_start: modulo 2^32, as k_cum)
   uint32_t q_cum, k_cum;
   uint32_t unused;
 };
@@ -46,8 +46,8 @@ struct phip_sequences {
   uint32_t n = 0;
   bool packed = false;
   uint32_t max_q = 0, max_k = 0;
-  uint32_t q_total = 0, k_total = 0;  // packed
-  uint64_t k_sum = 0;                 // keys of all sequences
+  uint32_t q_total = 0;  // packed
+  uint64_t k_sum = 0;    // keys of all sequences
 };
 
 namespace phip {

@@ -44,7 +44,7 @@ int create(phip_ctx *ctx, const uint32_t *q_lens, const uint32_t *k_lens, uint32
     places[i] = {entries[i].q_start, q_lens[i], (int32_t)k_lens[i] - (int32_t)q_lens[i], 0};
     q_at += q_lens[i];
     k_at += k_lens[i];
-    if (packed) PHIP_REQUIRE(q_at <= 0x7fffffffu && k_at <= 0x7fffffffu, "packed sequences of more than 2^31 - 1 tokens");
+    if (packed) PHIP_REQUIRE(q_at <= 0x7fffffffu, "packed sequences of more than 2^31 - 1 queries");
     max_q = std::max(max_q, q_lens[i]);
     max_k = std::max(max_k, k_lens[i]);
   }
@@ -65,7 +65,6 @@ int create(phip_ctx *ctx, const uint32_t *q_lens, const uint32_t *k_lens, uint32
   s->max_q = max_q;
   s->max_k = max_k;
   s->q_total = packed ? (uint32_t)q_at : 0;
-  s->k_total = packed ? (uint32_t)k_at : 0;
   s->k_sum = k_at;
   const int rc = phip_pool_alloc(ctx, (sizeof(SequenceEntry) + sizeof(SequencePlace)) * (size_t)n, &s->block, nullptr);
   if (rc != PHIP_OK) {
@@ -104,7 +103,8 @@ int sequence_view(phip_ctx *ctx, const phip_sequences *seqs, uint32_t tq, uint32
   if (seqs->packed) {
     PHIP_REQUIRE(bs == 1, "packed sequences lie in one sample, the tensors have %u", bs);
     PHIP_REQUIRE(seqs->q_total <= tq, "packed sequences of %u queries in %u tokens", seqs->q_total, tq);
-    PHIP_REQUIRE(!keys || seqs->k_total <= tk, "packed sequences of %u keys in %u tokens", seqs->k_total, tk);
+    // operators that read no keys take any number of them: the lengths are positions there
+    PHIP_REQUIRE(!keys || seqs->k_sum <= tk, "packed sequences of %llu keys in %u tokens", (unsigned long long)seqs->k_sum, tk);
   } else {
     PHIP_REQUIRE(seqs->n == bs, "%u sequences for %u samples", seqs->n, bs);
     PHIP_REQUIRE(seqs->max_q <= tq, "a sequence of %u queries in samples of %u tokens", seqs->max_q, tq);
@@ -112,7 +112,7 @@ int sequence_view(phip_ctx *ctx, const phip_sequences *seqs, uint32_t tq, uint32
   }
   const SequenceEntry *e = static_cast<const SequenceEntry *>(seqs->block);
   *out = {e, reinterpret_cast<const SequencePlace *>(e + seqs->n), seqs->n, tq, tk, seqs->packed ? 1u : 0u,
-          seqs->q_total, seqs->k_total};
+          seqs->q_total, keys && seqs->packed ? (uint32_t)seqs->k_sum : 0};
   return PHIP_OK;
 }
 

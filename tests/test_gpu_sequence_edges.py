@@ -572,3 +572,19 @@ def test_fp16_gradients_with_scores_of_hundreds(devices, shape, size):  # noqa: 
         r = getattr(want, n)
         assert np.abs(r).max() < 65504
         check(n, x.to_vector(), r, getattr(want, "tol_" + n) + (step if n in ("gq", "gk") else 0))
+
+
+def test_packed_tokens_at_far_positions(devices):  # noqa: F811
+    """The lengths of keys are positions to the rotary operators: their sum has no limit.  Attention needs the keys."""
+    dev = devices["f32"]
+    rng = np.random.default_rng(24)
+    q_lens, k_lens = (2, 3, 1), (2 ** 31 - 1, 2 ** 31 - 5, 2 ** 30)
+    x, freqs = draw(rng, "f32", 1, 6, 2, 64), pa.rotary_frequencies(32)[0]
+    lists = dev.new_sequences(q_lens, k_lens, True)
+    y, _ = dev.rotary_fw(tensor(dev, x), None, freqs, seqs=lists)
+    want = Rotary(x, places(1, 6, 6, q_lens, k_lens, True), freqs, "f32")
+    # the angle's product, in 64 bits: half a step each of it and of the turns, at 2^31 radians 2^-21 in all
+    check("y", y.to_vector(), want.y, want.tol_y + 2.0 ** -21 * np.abs(x).max() * 2)
+    t = tensor(dev, x)
+    with pytest.raises(pa.Error, match="packed sequences"):
+        dev.attention_fw(t, t, t, seqs=lists)
