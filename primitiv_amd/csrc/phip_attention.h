@@ -168,7 +168,8 @@ __device__ inline Frag<T> load_frag(const T *row, bool valid, int d0, int d) {
   if constexpr (sizeof(T) == 2) {
     return {load_part<WHOLE, TINY>(row, valid && d0 < d, d0, d)};
   } else {
-    const u32x4 lo = load_part<WHOLE, TINY>(row, valid && d0 < d, d0, d), hi = load_part<WHOLE, TINY>(row, valid && d0 + 4 < d, d0 + 4, d);
+    const u32x4 lo = load_part<WHOLE, TINY>(row, valid && d0 < d, d0, d);
+    const u32x4 hi = load_part<WHOLE, TINY>(row, valid && d0 + 4 < d, d0 + 4, d);
     f32x8 f;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
@@ -525,8 +526,7 @@ inline uint64_t slots(const SequenceView &s, uint32_t size, uint32_t rows_per, b
   return total * rows_per / size + s.n + ((tokens - total) * rows_per + size - 1) / size;
 }
 
-// ---- arguments ------------------------------------------------------------------------------------------------------
-
+// ---- which kernel ---------------------------------------------------------------------------------------------------
 
 // Stages of a wavefront's own ring of pairs of 32-row tiles: four wavefronts take 128 KiB of LDS at most.
 template <typename T, int DP>
@@ -552,7 +552,8 @@ constexpr int kStages = 32 * Tile<T, DP>::kPitch <= 8192 ? 2 : 1;
 //   64 tokens, 16 of 64          40 -> 43       69 -> 52       240 -> 196  (forward alone 43 -> 51)
 //   96 tokens, 16 of 64          52 -> 54       92 -> 62       253 -> 221
 //   128 tokens, 16 of 64         64 -> 65       70 -> 73       233 -> 250
-// Walks of more than 256 keys (rows) want the 1024 tiles too: 4 queries, 500 keys, 8 heads of 128, forward: 58 -> 84 and 117 -> 96.
+// Walks of more than 256 keys (rows) want the 1024 tiles too: 4 queries, 500 keys, 8 heads of 128, forward: 58 -> 84 and
+// 117 -> 96.
 enum class Way { Shared, Four, One };
 // wide, narrow: workgroups with tiles of 128 and of 32; most: rows (keys) of the longest sequence; walked: what its
 // workgroups walk over.

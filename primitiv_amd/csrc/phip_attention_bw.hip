@@ -754,7 +754,8 @@ struct Plan {
     Way way;
     uint64_t wide, narrow;  // with tiles of 128, of 32
     bool launchable() const {
-      return way == Way::Shared ? attention::launchable(wide, kThreads) : attention::launchable(narrow, way == Way::One ? 64 : 256);
+      return way == Way::Shared ? attention::launchable(wide, kThreads)
+                                : attention::launchable(narrow, way == Way::One ? 64 : 256);
     }
   };
   Side q, k;
@@ -763,7 +764,8 @@ struct Plan {
 
 template <typename T>
 Plan make_plan(phip_ctx *ctx, const BwArgs<T> &a, const phip_sequences *seqs) {
-  const uint64_t most_q = (uint64_t)(seqs != nullptr ? seqs->max_q : a.seq.tq) * a.s.g, most_k = seqs != nullptr ? seqs->max_k : a.seq.tk;
+  const uint64_t most_q = (uint64_t)(seqs != nullptr ? seqs->max_q : a.seq.tq) * a.s.g;
+  const uint64_t most_k = seqs != nullptr ? seqs->max_k : a.seq.tk;
   Plan p = {{Way::Shared, slots(a.seq, 128, a.s.g, false) * a.s.hk, slots(a.seq, 32, a.s.g, false) * a.s.hk},
             {Way::Shared, slots(a.seq, 128, 1, true) * a.s.hk, slots(a.seq, 32, 1, true) * a.s.hk},
             most_k};

@@ -27,7 +27,6 @@ struct FwArgs {
   uint32_t chunk;
   uint32_t splits;      // ranges of the longest sequence; a workgroup for each range of each tile, or,
   uint32_t listed;      // if not 0: workgroups for the ranges that the listed sequences have (see find_range): their slots
-  uint32_t exact;       // probabilities in two parts
   uint32_t part_rows;   // rows of a tile that exist at most
   float *partial;       // per tile and range: part_rows x (DP sums, maximum, sum, 2 unused)
   uint32_t *tickets;
@@ -170,26 +169,29 @@ __device__ inline Frag16<T> left_out(const f32x16 &p, int c, const Frag16<T> &f)
   return r;
 }
 
-// The product with the values.  exact (16-bit storage): the probabilities in two parts, which together carry 16 bits (bf16) or
+// The product with the values.  EXACT (16-bit storage): the probabilities in two parts, which together carry 16 bits (bf16) or
 // 22 (fp16).  Taken where a sequence's rows are one tile, the single tokens of a serving loop: those calls wait for memory, so
-// the second product costs 1 to 5 % (one token of 31 streams of 4096 keys, 32/8 heads of 128, bf16: 95 -> 96 us; 130001 keys,
-// fp16: 105 -> 106) and the result is as far from the exact one as its own rounding (root mean square error 1.27 and 1.33 ->
-// 1.0 times that).  Prompts are bound by the products and the vector instructions and take one part.
-template <typename T, int DP, int KB>
-__device__ inline void values(Rows<DP> &st, const Scores<KB> &sc, uint32_t v_at, bool exact) {
+// the second product costs 1 to 2 % (one token of 16 streams of 1 to 8192 keys, 32/8 heads of 128, bf16: 55.1 -> 56.2 us; 130001
+// keys, fp16: 104.2 -> 105.1) and the result is as far from the exact one as its own rounding (root mean square error 1.27 and
+// 1.33 -> 1.0 times that).  Prompts are bound by the products and the vector instructions and take one part.
+template <typename T, int DP, int KB, bool EXACT>
+__device__ inline void values(Rows<DP> &st, const Scores<KB> &sc, uint32_t v_at) {
 #pragma unroll
   for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
       const Frag<T> p = as_operand(sc.s[kb], c, (Frag<T> *)nullptr);
+      if constexpr (EXACT) {
+        const Frag<T> rest = left_out<T>(sc.s[kb], c, p);
 #pragma unroll
-      for (int db = 0; db < DP / 32; ++db) mma(st.o[db], Tile<T, DP>::col_frag(v_at, 2 * kb + c, db), p);
-      if constexpr (sizeof(T) == 2) {
-        if (exact) {
-          const Frag<T> rest = left_out<T>(sc.s[kb], c, p);
-#pragma unroll
-          for (int db = 0; db < DP / 32; ++db) mma(st.o[db], Tile<T, DP>::col_frag(v_at, 2 * kb + c, db), rest);
+        for (int db = 0; db < DP / 32; ++db) {
+          const Frag<T> v = Tile<T, DP>::col_frag(v_at, 2 * kb + c, db);
+          mma(st.o[db], v, p);
+          mma(st.o[db], v, rest);
         }
+      } else {
+#pragma unroll
+        for (int db = 0; db < DP / 32; ++db) mma(st.o[db], Tile<T, DP>::col_frag(v_at, 2 * kb + c, db), p);
       }
     }
 }
@@ -300,7 +302,7 @@ __global__ __launch_bounds__(kThreads, 2) void rows_kernel(const FwArgs<T> a) {
       softmax<T, DP, KT / 32>(st, sc, t * KT, lim, (t + 1) * KT > w_all, sh.scale_log2, lane);
       const bool masked = (t + 1) * KT > w_all;
       if (!masked || !values_masked<T, DP, KT / 32>(st, sc, stage + kTile + col_at, t * KT, lim, lane))
-        values<T, DP, KT / 32>(st, sc, stage + kTile + col_at, false);
+        values<T, DP, KT / 32, false>(st, sc, stage + kTile + col_at);
     }
   }
 
@@ -363,7 +365,8 @@ __device__ inline RangePlace find_range(const FwArgs<T> &a, uint32_t index, uint
   const Shape &sh = a.s;
   if (a.listed == 0) {
     const uint32_t slot = index / a.splits, tile = slot * sh.hk + head;
-    return {find_place(a.seq, slot, a.tiles, 32, sh.g, false, sh.causal != 0), index - slot * a.splits, tile * a.splits, 1, tile};
+    return {find_place(a.seq, slot, a.tiles, 32, sh.g, false, sh.causal != 0), index - slot * a.splits, tile * a.splits, 1,
+            tile};
   }
   const uint32_t slot = index / a.tiles, t = index - slot * a.tiles;
   if (slot >= a.listed)
@@ -385,7 +388,7 @@ __device__ inline RangePlace find_range(const FwArgs<T> &a, uint32_t index, uint
           a.tiles * sh.hk, (lo * a.tiles + t) * sh.hk + head};
 }
 
-template <typename T, int DP, bool DMA, int W>
+template <typename T, int DP, bool DMA, int W, bool EXACT>
 __global__ __launch_bounds__(64 * W, 1) void few_kernel(const FwArgs<T> a) {
   constexpr int BM = 32, S = kStages<T, DP>, kThreads = 64 * W;
   typedef Tile<T, DP> L;
@@ -465,7 +468,7 @@ __global__ __launch_bounds__(64 * W, 1) void few_kernel(const FwArgs<T> a) {
       softmax<T, DP, 1>(st, sc, key, lim, key + 32 > all, sh.scale_log2, lane);
       wait_loads<kInFlight>();
       if (key + 32 <= first_sees || !values_masked<T, DP, 1>(st, sc, stage + kTile + col_at, key, lim, lane))
-        values<T, DP, 1>(st, sc, stage + kTile + col_at, a.exact != 0);
+        values<T, DP, 1, EXACT>(st, sc, stage + kTile + col_at);
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
       fetch_v(key + S * kStep, s);
     }
@@ -486,7 +489,7 @@ __global__ __launch_bounds__(64 * W, 1) void few_kernel(const FwArgs<T> a) {
       scores<T, DP, 1>(sc, qf, ring + row_at);
       softmax<T, DP, 1>(st, sc, key, lim, key + 32 > all, sh.scale_log2, lane);
       if (key + 32 <= first_sees || !values_masked<T, DP, 1>(st, sc, ring + kTile + col_at, key, lim, lane))
-        values<T, DP, 1>(st, sc, ring + kTile + col_at, a.exact != 0);
+        values<T, DP, 1, EXACT>(st, sc, ring + kTile + col_at);
     }
   }
 
@@ -625,10 +628,10 @@ uint32_t few_chunk(phip_ctx *ctx, const SequenceView &view, const phip_sequences
   return (uint32_t)std::min<uint64_t>((std::max<uint64_t>(share, 256) + 127) / 128 * 128, 1u << 30);
 }
 
-template <typename T, int DP, bool DMA, int W>
+template <typename T, int DP, bool DMA, int W, bool EXACT = false>
 int launch_few(phip_ctx *ctx, FwArgs<T> a, const phip_sequences *seqs) {
   constexpr int lds = kFewLds<T, DP, W>;
-  const int rc = allow_lds<few_kernel<T, DP, DMA, W>>(ctx, lds);
+  const int rc = allow_lds<few_kernel<T, DP, DMA, W, EXACT>>(ctx, lds);
   if (rc != PHIP_OK) return rc;
   a.tiles = (uint32_t)(((uint64_t)a.seq.tq * a.s.g + 31) / 32);
   const uint64_t tiles = slots(a.seq, 32, a.s.g, false) * a.s.hk;
@@ -638,7 +641,6 @@ int launch_few(phip_ctx *ctx, FwArgs<T> a, const phip_sequences *seqs) {
   uint64_t blocks = tiles * a.splits, parts = blocks;
   const uint64_t most_rows = std::max<uint64_t>(1, (uint64_t)(a.seq.packed ? seqs->max_q : a.seq.tq) * a.s.g);
   a.part_rows = (uint32_t)std::min<uint64_t>(32, most_rows);
-  a.exact = sizeof(T) == 2 && most_rows <= 32 ? 1 : 0;
   if (a.splits > 1 && seqs != nullptr && seqs->k_sum <= 0xffffffffu) {
     // One long sequence among many short ones: its ranges times all tiles would be mostly empty workgroups, each with a place
     // in the scratch memory (131072 keys beside 127 times 64, one key head: 512 MB and 137 us; listed 4 MB and 62 us).  With
@@ -661,7 +663,7 @@ int launch_few(phip_ctx *ctx, FwArgs<T> a, const phip_sequences *seqs) {
     a.partial = static_cast<float *>(partial);
     a.tickets = tile_tickets(ctx);
   }
-  hipLaunchKernelGGL((few_kernel<T, DP, DMA, W>), dim3((uint32_t)blocks), dim3(64 * W), lds, ctx->stream, a);
+  hipLaunchKernelGGL((few_kernel<T, DP, DMA, W, EXACT>), dim3((uint32_t)blocks), dim3(64 * W), lds, ctx->stream, a);
   const hipError_t e = hipGetLastError();
   if (partial != nullptr) phip_pool_free(ctx, partial);
   if (e != hipSuccess) return fail(PHIP_ERR_RUNTIME, "launching the attention kernel failed: %s", hipGetErrorString(e));
@@ -678,7 +680,12 @@ int launch(phip_ctx *ctx, const FwArgs<T> &a, const phip_sequences *seqs) {
   if constexpr (sizeof(T) == 4) {
     if (way == Way::One) return launch_few<T, DP, DMA, 1>(ctx, a, seqs);
   }
-  if (way == Way::Four) return launch_few<T, DP, DMA, 4>(ctx, a, seqs);
+  if (way == Way::Four) {
+    if constexpr (sizeof(T) == 2) {  // a tile per sequence
+      if ((a.seq.packed ? most : (uint64_t)a.seq.tq * a.s.g) <= 32) return launch_few<T, DP, DMA, 4, true>(ctx, a, seqs);
+    }
+    return launch_few<T, DP, DMA, 4>(ctx, a, seqs);
+  }
   return launch_rows<T, DP, DMA>(ctx, a);
 }
 
