@@ -222,7 +222,7 @@ __device__ inline void store_row(T *row, const f32x16 (&x)[DP / 32], float f, bo
 // Many rows: a workgroup of four wavefronts takes 128 rows, 32 per wavefront, and walks over the keys in tiles of KT.
 // Tile t + 1 is on its way while tile t is worked on (two stages of K and V, one barrier per tile; 64 KiB of LDS and at most
 // 256 registers, so that two workgroups share a CU and one's products run beside the other's exponentials).
-// Bound by the two pipes: 16 Ki packed tokens, 32/8 heads of 128, bf16, causal: 871 us, 940 TFLOP/s, the matrix pipe busy 44 %
+// Bound by the two pipes: 16 Ki packed tokens, 32/8 heads of 128, bf16, causal: 889 us, 920 TFLOP/s, the matrix pipe busy 43 %
 // and the vector pipe 51 % of the time (an exponential per score costs about what its 4 x 128 flops do); fp32, 8 x 2048
 // tokens, 16 heads of 64: 556 us, 124 TFLOP/s of the 139 that a large product reaches.
 template <typename T>
@@ -319,8 +319,8 @@ __global__ __launch_bounds__(kThreads, 2) void rows_kernel(const FwArgs<T> a) {
 //
 // Every wavefront has a ring of LDS tiles of its own and waits for nobody else: K and V blocks alternate in it, and the
 // block `kRing` positions ahead is ordered as soon as a block has been used, so that up to three quarters of 128 KiB are on
-// their way to every CU.  Bound by memory: one token against 130001 keys, 8 key heads of 128, fp16: 104 us, 5.1 TB/s, the
-// rate of a large copy; one token of 16 streams against 1 to 8192 keys: 55 us, 4.0 TB/s.
+// their way to every CU.  Bound by memory: one token against 130001 keys, 8 key heads of 128, fp16: 105 us, 5.1 TB/s, the
+// rate of a large copy; one token of 16 streams against 1 to 8192 keys: 56 us, 3.9 TB/s.
 template <typename T, int DP, int W>
 constexpr int kFewLds = W * std::max(2 * kStages<T, DP> * 32 * Tile<T, DP>::kPitch, (DP * 33 + 64) * 4);
 
